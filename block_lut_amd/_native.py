@@ -23,6 +23,7 @@ LUTMOE_EALIGN = -5
 FMT_REF = 0
 FMT_BL4 = 1
 FMT_NESTED = 2
+FMT_MXFP4 = 3
 
 QRULE_QUANTIZER = 0
 QRULE_MIDPOINTS = 1
@@ -38,6 +39,8 @@ STAGE_ALL = 7
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_F16 = 2
+DTYPE_MXFP4 = 3
 
 
 class LutMoeNotBuilt(RuntimeError):
@@ -124,6 +127,11 @@ PROTOTYPES = {
     "lutmoe_moe_forward_logits_ex": (I32, [DP, P, P, I32, I32, I32, F32, P, I32, P, SZ, I32, I32, P]),
     "lutmoe_moe_forward_noalloc": (I32, [DP, P, P, P, I32, I32, P, I32, I32, P]),
     "lutmoe_noalloc_prepare": (I32, []),
+    "lutmoe_grouped_gemm": (I32, [P, I32, P, P, I32, I32, I32, I32, P, I32, I32, P]),
+    "lutmoe_grouped_gemm_dgrad": (I32, [P, I32, P, P, I32, I32, I32, I32, P, I32, I32, P]),
+    "lutmoe_grouped_gemm_wgrad": (I32, [P, I32, P, P, I32, I32, I32, I32, P, I32, P]),
+    "lutmoe_grouped_gemm_mxfp4": (I32, [WP, P, I32, P, P, I32, P, I32, I32, P]),
+    "lutmoe_mxfp4_encode": (I32, [P, I32, I64, P, P, P]),
     "lutmoe_bl4_encode": (I32, [P, I64, I32, P, P, P]),
     "lutmoe_ref_encode": (I32, [P, P, I64, I32, P, P, P]),
 }

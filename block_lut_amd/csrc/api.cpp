@@ -61,6 +61,10 @@ int validate_weights(const lutmoe_weights* w) {
         case LUTMOE_FMT_NESTED:
             if (w->cols % 64 || !w->tier_bits) return LUTMOE_EINVAL;
             return LUTMOE_OK;
+        case LUTMOE_FMT_MXFP4:
+            if (w->cols % 32) return LUTMOE_EINVAL;
+            if (!aligned(w->codes, 16)) return LUTMOE_EALIGN;
+            return LUTMOE_OK;
         default:
             return LUTMOE_EINVAL;
     }
@@ -137,7 +141,7 @@ int validate_moe(const lutmoe_moe_desc* d) {
         return LUTMOE_EINVAL;
     const int E_tot = d->num_routed + d->num_shared;
     if (d->w13.num_experts < E_tot || d->w2.num_experts < E_tot) return LUTMOE_EINVAL;
-    if (d->w13.format != d->w2.format) return LUTMOE_EUNSUPPORTED;
+    if (d->w13.format != d->w2.format || d->w13.format == LUTMOE_FMT_MXFP4) return LUTMOE_EUNSUPPORTED;
     if (H % 64 || I % 64) return LUTMOE_EUNSUPPORTED;
     if (d->shared_gate && !aligned(d->shared_gate, 16)) return LUTMOE_EALIGN;
     if (d->dense_inter < 0 || d->dense_reserved != 0) return LUTMOE_EINVAL;
@@ -151,6 +155,45 @@ int validate_moe(const lutmoe_moe_desc* d) {
         if ((rc = validate_ref_vector(&d->w13)) || (rc = validate_ref_vector(&d->w2))) return rc;
     }
     return LUTMOE_OK;
+}
+
+// Sizes that the grouped products take.
+int validate_grouped(int E, int P, int M, int K) {
+    if (E <= 0 || P < 0 || M <= 0 || K <= 0) return LUTMOE_EINVAL;
+    if (E > 4096 || M > (1 << 20) || K > (1 << 20)) return LUTMOE_EUNSUPPORTED;
+    return LUTMOE_OK;
+}
+
+size_t out_align(int dtype) { return dtype == LUTMOE_DTYPE_F32 ? 4 : 2; }
+
+// a: rows [P][..] (x, or dy), b: the other operand; rows are read only where P > 0
+int grouped_dense(int op, const void* a, int dtype, const void* b, const int32_t* offsets, int E, int P, int M, int K,
+                  void* out, int out_dtype, int zero_rest, hipStream_t s) {
+    int rc = validate_grouped(E, P, M, K);
+    if (rc) return rc;
+    if (dtype != LUTMOE_DTYPE_BF16 && dtype != LUTMOE_DTYPE_F16) return LUTMOE_EINVAL;
+    if (out_dtype != dtype && out_dtype != LUTMOE_DTYPE_F32) return LUTMOE_EINVAL;
+    if (M % 8 || K % 8) return LUTMOE_EUNSUPPORTED;
+    if (P == 0 && op != lutmoe::kGroupedWgrad) return LUTMOE_OK;
+    if (!offsets || !out || (P > 0 && (!a || !b))) return LUTMOE_EINVAL;
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(out, out_align(out_dtype)) || !aligned(offsets, 4))
+        return LUTMOE_EALIGN;
+    GroupedArgs g{op, E, P, M, K, offsets, a, nullptr, dtype, b, nullptr, out, out_dtype, aligned(out, 16),
+                  zero_rest ? 1 : 0};
+    return launch_grouped(g, s);
+}
+
+// offsets NULL: one group of all rows (w has one matrix)
+int grouped_mxfp4(const lutmoe_weights* w, const void* x, int x_dtype, const uint8_t* x_scales, const int32_t* offsets,
+                  int P, void* y, int y_dtype, int zero_rest, hipStream_t s) {
+    int rc = validate_grouped(w->num_experts, P, w->rows, w->cols);
+    if (rc) return rc;
+    if (P == 0) return LUTMOE_OK;
+    if (!x || !y) return LUTMOE_EINVAL;
+    if (!aligned(x, 16) || !aligned(y, out_align(y_dtype)) || (offsets && !aligned(offsets, 4))) return LUTMOE_EALIGN;
+    GroupedArgs g{lutmoe::kGroupedFwd, w->num_experts, P, w->rows, w->cols, offsets, x, x_scales, x_dtype, w->codes,
+                  w->tables, y, y_dtype, w->rows % 8 == 0 && aligned(y, 16), zero_rest ? 1 : 0};
+    return launch_grouped(g, s);
 }
 
 }  // namespace
@@ -316,6 +359,10 @@ int lutmoe_dequant(const lutmoe_weights* w, int e0, int ne, void* out, void* str
                                       (const uint16_t*)w->tables + e0 * (n / 4), ne * nbl,
                                       stream_of(stream));
         }
+        case LUTMOE_FMT_MXFP4:
+            if (!aligned(out, 16)) return LUTMOE_EALIGN;
+            return launch_mxfp4_dequant((uint16_t*)out, (const uint8_t*)w->codes + e0 * (n / 2),
+                                        (const uint8_t*)w->tables + e0 * (n / 32), ne * (n / 32), stream_of(stream));
         default:
             if (!aligned(out, 16)) return LUTMOE_EALIGN;
             return launch_nested_dequant((uint16_t*)out, w, e0, ne, stream_of(stream));
@@ -331,6 +378,15 @@ int lutmoe_gemv_ex(const lutmoe_weights* w, int expert, const void* x, int x_dty
     if (x_dtype != LUTMOE_DTYPE_BF16 && x_dtype != LUTMOE_DTYPE_F32) return LUTMOE_EINVAL;
     if (!aligned(x, 16) || w->cols % 8) return LUTMOE_EALIGN;
     if (T == 0) return LUTMOE_OK;
+    if (w->format == LUTMOE_FMT_MXFP4) {   // one group of all T rows
+        if (x_dtype == LUTMOE_DTYPE_F32) return LUTMOE_EUNSUPPORTED;
+        lutmoe_weights one = *w;
+        const int64_t n = (int64_t)w->rows * w->cols;
+        one.num_experts = 1;
+        one.codes = (const uint8_t*)w->codes + expert * (n / 2);
+        one.tables = (const uint8_t*)w->tables + expert * (n / 32);
+        return grouped_mxfp4(&one, x, LUTMOE_DTYPE_BF16, nullptr, nullptr, T, y, y_dtype, 0, stream_of(stream));
+    }
     if (w->format == LUTMOE_FMT_NESTED) {
         if (x_dtype == LUTMOE_DTYPE_F32) return LUTMOE_EUNSUPPORTED;
         return launch_nested_gemv(w, expert, (const uint16_t*)x, T, y, y_dtype, stream_of(stream));
@@ -380,6 +436,36 @@ int lutmoe_permute(const int32_t* topk_ids, int T, int k, int E, int32_t* offset
     if (!topk_ids || !offsets || !perm || !inv || !active) return LUTMOE_EINVAL;
     if ((int64_t)T * k >= (1ll << 31)) return LUTMOE_EUNSUPPORTED;
     return launch_permute(topk_ids, T, k, E, offsets, perm, inv, active, stream_of(stream));
+}
+
+// ------------------------------------------------------- grouped products
+
+int lutmoe_grouped_gemm(const void* x, int dtype, const void* w, const int32_t* offsets, int E, int P, int M, int K,
+                        void* y, int y_dtype, int zero_rest, void* stream) {
+    return grouped_dense(lutmoe::kGroupedFwd, x, dtype, w, offsets, E, P, M, K, y, y_dtype, zero_rest, stream_of(stream));
+}
+
+int lutmoe_grouped_gemm_dgrad(const void* dy, int dtype, const void* w, const int32_t* offsets, int E, int P, int M,
+                              int K, void* dx, int dx_dtype, int zero_rest, void* stream) {
+    return grouped_dense(lutmoe::kGroupedDgrad, dy, dtype, w, offsets, E, P, M, K, dx, dx_dtype, zero_rest,
+                         stream_of(stream));
+}
+
+int lutmoe_grouped_gemm_wgrad(const void* dy, int dtype, const void* x, const int32_t* offsets, int E, int P, int M,
+                              int K, void* dw, int dw_dtype, void* stream) {
+    return grouped_dense(lutmoe::kGroupedWgrad, dy, dtype, x, offsets, E, P, M, K, dw, dw_dtype, 0, stream_of(stream));
+}
+
+int lutmoe_grouped_gemm_mxfp4(const lutmoe_weights* w, const void* x, int x_dtype, const uint8_t* x_scales,
+                              const int32_t* offsets, int P, void* y, int y_dtype, int zero_rest, void* stream) {
+    const int rc = validate_weights(w);
+    if (rc) return rc;
+    if (w->format != LUTMOE_FMT_MXFP4) return LUTMOE_EUNSUPPORTED;
+    if (y_dtype != LUTMOE_DTYPE_BF16 && y_dtype != LUTMOE_DTYPE_F32) return LUTMOE_EINVAL;
+    if (x_dtype != LUTMOE_DTYPE_BF16 && x_dtype != LUTMOE_DTYPE_MXFP4) return LUTMOE_EINVAL;
+    if ((x_dtype == LUTMOE_DTYPE_MXFP4) != (x_scales != nullptr) && P > 0) return LUTMOE_EINVAL;
+    if (!offsets && P > 0) return LUTMOE_EINVAL;
+    return grouped_mxfp4(w, x, x_dtype, x_scales, offsets, P, y, y_dtype, zero_rest, stream_of(stream));
 }
 
 // -------------------------------------------------------------- MoE layer
@@ -626,6 +712,15 @@ int lutmoe_bl4_encode(const float* w, int64_t nblocks, int n_iter, uint8_t* code
     if (nblocks == 0) return LUTMOE_OK;
     if (!w || !codes || !tables_f16) return LUTMOE_EINVAL;
     return launch_bl4_encode(w, nblocks, n_iter, codes, tables_f16, stream_of(stream));
+}
+
+int lutmoe_mxfp4_encode(const void* x, int x_dtype, int64_t nblocks, uint8_t* codes, uint8_t* scales, void* stream) {
+    if (nblocks < 0) return LUTMOE_EINVAL;
+    if (x_dtype != LUTMOE_DTYPE_BF16 && x_dtype != LUTMOE_DTYPE_F16 && x_dtype != LUTMOE_DTYPE_F32) return LUTMOE_EINVAL;
+    if (nblocks == 0) return LUTMOE_OK;
+    if (!x || !codes || !scales) return LUTMOE_EINVAL;
+    if (!aligned(x, 16) || !aligned(codes, 16)) return LUTMOE_EALIGN;
+    return launch_mxfp4_encode(x, x_dtype, nblocks, codes, scales, stream_of(stream));
 }
 
 int lutmoe_kmeans_1d(const float* data, int64_t n, float* centroids, int k, int n_iter, int32_t* assign_ws,

@@ -18,7 +18,8 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "liblutmoe.so")
 SOURCES = ["api.cpp", "dequant.hip", "gemv.hip", "decode.hip", "route.hip", "gemm.hip",
-           "encode.hip", "noalloc.hip", "dense.hip", "stream.hip"]
+           "encode.hip", "noalloc.hip", "dense.hip", "stream.hip",
+           "mxfp4.hip", "grouped.hip"]
 ARCH = "gfx950"
 
 

@@ -18,6 +18,9 @@ struct RouteChunks {
     int cn[kMaxChunks];
 };
 
+// grouped.hip: which product
+constexpr int kGroupedFwd = 0, kGroupedDgrad = 1, kGroupedWgrad = 2;
+
 }  // namespace lutmoe
 
 namespace lutmoe_host {
@@ -171,5 +174,26 @@ int launch_bl4_encode(const float* w, int64_t nblocks, int n_iter, uint8_t* code
 int launch_kmeans_1d(const float* x, int64_t n, float* cent, int k, int n_iter, int32_t* asg, hipStream_t s);
 int launch_ref_encode(const uint16_t* w, const float* codebook, int64_t n, int block_size, uint8_t* codes,
                       uint16_t* absmax, hipStream_t s);
+
+// mxfp4.hip
+int launch_mxfp4_encode(const void* x, int dtype, int64_t nblocks, uint8_t* codes, uint8_t* scales, hipStream_t s);
+int launch_mxfp4_dequant(uint16_t* out, const uint8_t* codes, const uint8_t* scales, int64_t nblocks, hipStream_t s);
+
+// grouped.hip: products of rows sorted by expert.
+struct GroupedArgs {
+    int op;                    // kGroupedFwd / Dgrad / Wgrad
+    int E, P, M, K;            // matrices [M][K], rows
+    const int32_t* offsets;    // [E + 1]; NULL: one group of all rows (E = 1)
+    const void* x;             // forward: [P][K], gradients: dy [P][M]
+    const void* x_scales;      // MXFP4 rows: scale bytes [P][K / 32], else NULL
+    int x_dtype;
+    const void* w;             // forward and dgrad: [E][M][K]; wgrad: x [P][K]
+    const void* w_scales;      // MXFP4 matrices: scale bytes [E][M][K / 32], else NULL
+    void* out;                 // [P][M], [P][K] or [E][M][K]
+    int out_dtype;
+    bool out_vec;              // rows of the result are 16-byte aligned
+    int zero_rest;             // forward, dgrad: rows of no group are set to zero (else not written)
+};
+int launch_grouped(const GroupedArgs& g, hipStream_t s);
 
 }  // namespace lutmoe_host

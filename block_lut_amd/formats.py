@@ -11,6 +11,8 @@ BL4  (4-bit, per-64-block codebooks): codes uint8 [E, M, K/2] (even element in
 NL   (NestedLUT 2/3/4-bit tiers): per expert, bit-plane sections
      [p01 | p2 | p3] (a tier-b expert keeps the first 2, 3 or all of them) and
      a bf16 table [M, K/64, 2^b].
+MXFP4 (blocks of 32 along K): codes uint8 [E, M, K/2] (E2M1 elements, even one in
+     the low nibble), scales uint8 [E, M, K/32] (byte b: 2^(b - 127), 255: NaN).
 """
 from __future__ import annotations
 
@@ -142,6 +144,47 @@ class BL4Stack(WeightStack):
 
     def hbm_bytes_per_expert(self) -> int:
         return self.rows * self.cols // 2 + self.rows * (self.cols // 64) * 32
+
+
+class MXFP4Stack(WeightStack):
+    """4-bit floating point elements with a power-of-two scale per 32 (``ops.mxfp4_encode``
+    makes both).  For ``ops.dequant``, ``ops.gemv`` and ``ops.grouped_gemm``; the fused MoE
+    layer does not take it."""
+
+    format = N.FMT_MXFP4
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dim() == 2:
+            codes = codes.unsqueeze(0)
+        if scales.dim() == 2:
+            scales = scales.unsqueeze(0)
+        self.codes = _dev(codes, torch.uint8, "codes")
+        self.scales = _dev(scales, torch.uint8, "scales")
+        if codes.dim() != 3:
+            raise ValueError("MXFP4 codes must be [E, M, K/2] or [M, K/2]")
+        E, M, Kh = self.codes.shape
+        if not (E and M and Kh) or Kh % 16:
+            raise ValueError("MXFP4 needs at least one row and K % 32 == 0")
+        if tuple(self.scales.shape) != (E, M, Kh // 16):
+            raise ValueError(f"scales shape {tuple(self.scales.shape)} != {(E, M, Kh // 16)}")
+        if self.scales.device != self.codes.device:
+            raise ValueError("codes and scales must be on the same device")
+        self.num_experts, self.rows, self.cols = E, M, 2 * Kh
+
+    def desc(self) -> N.lutmoe_weights:
+        d = N.lutmoe_weights()
+        d.format = N.FMT_MXFP4
+        d.num_experts, d.rows, d.cols = self.num_experts, self.rows, self.cols
+        d.codes = self.codes.data_ptr()
+        d.tables = self.scales.data_ptr()
+        d.codebook = None
+        d.tier_bits = None
+        d.absmax_per_expert = 0
+        d.block_size = 32
+        return d
+
+    def hbm_bytes_per_expert(self) -> int:
+        return self.rows * self.cols // 2 + self.rows * (self.cols // 32)
 
 
 @dataclass
@@ -344,6 +387,12 @@ def split_shared_ref(codes13: torch.Tensor, absmax13: torch.Tensor, codes2: torc
 # from torch.cuda.current_stream() where torch has no such handle
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _raw_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _here(t: torch.Tensor) -> bool:
+    """Whether ``t`` is on the current device."""
+    current = torch.cuda.current_device() if _raw_device is None else _raw_device()
+    return t.get_device() == current
 
 
 def _stream() -> int:

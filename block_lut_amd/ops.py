@@ -7,12 +7,12 @@ no CPU or PyTorch fallback: a missing library raises ``LutMoeNotBuilt``.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _native as N
-from .formats import MoEWeights, WeightStack, _dev, _stream
+from .formats import MXFP4Stack, MoEWeights, WeightStack, _dev, _here, _stream
 
 _DT = {torch.bfloat16: N.DTYPE_BF16, torch.float32: N.DTYPE_F32}
 
@@ -224,6 +224,165 @@ def permute(topk_ids: torch.Tensor, num_experts: int):
     return offsets, perm, inv, active
 
 
+# -------------------------------------------------------- grouped products
+
+_GROUPED_DT = {torch.bfloat16: N.DTYPE_BF16, torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16}
+
+
+def _grouped_rows(t: torch.Tensor, dtype: torch.dtype, name: str, offsets: torch.Tensor, experts: int) -> int:
+    """Checks of the rows and offsets of a grouped product; the number of rows."""
+    _dev(t, dtype, name)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
+    _dev(offsets, torch.int32, "offsets")
+    if offsets.numel() != experts + 1:
+        raise ValueError(f"offsets must hold {experts + 1} values (one more than the experts)")
+    if offsets.device != t.device:
+        raise ValueError("offsets and rows must be on the same device")
+    return t.shape[0]
+
+
+def _grouped_weights(w: torch.Tensor, dtype: torch.dtype, device: torch.device) -> Tuple[int, int, int]:
+    _dev(w, dtype, "w")
+    if w.dim() != 3:
+        raise ValueError("w must be [E, M, K]")
+    if w.device != device:
+        raise ValueError("w and rows must be on the same device")
+    return tuple(w.shape)
+
+
+def _grouped_out(out: Optional[torch.Tensor], dtype: torch.dtype, shape: Tuple[int, ...], device: torch.device):
+    """The result tensor: ``out``, checked, or a new one."""
+    if dtype not in _GROUPED_DT:
+        raise TypeError(f"the result must be bfloat16, float16 or float32, got {dtype}")
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _dev(out, dtype, "out")
+    if tuple(out.shape) != shape or out.device != device:
+        raise ValueError(f"out must be {shape} on {device}")
+    return out
+
+
+def grouped_gemm(x: torch.Tensor, w: Union[torch.Tensor, MXFP4Stack], offsets: torch.Tensor,
+                 x_scales: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Rows times their expert's matrix: y[p] = x[p] . W[e]^T for offsets[e] <= p <
+    offsets[e + 1] (int32 [E + 1] on the device, as ``permute`` gives them; offsets[0] is 0).
+
+    x [P, K] and w [E, M, K] in bf16 or fp16 (M and K multiples of 8); or w an ``MXFP4Stack``
+    and x bf16, or x uint8 codes [P, K/2] with ``x_scales`` [P, K/32] (``mxfp4_encode``).
+    fp32 accumulation, the result rounded once to ``out_dtype`` (default: x's, bf16 for
+    MXFP4; or fp32).  Rows behind the last group are zero in a result made here, and left as
+    they were in ``out``.  Not differentiable (``grouped_linear`` is)."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and not _here(x):
+        with torch.cuda.device(x.device):
+            return grouped_gemm(x, w, offsets, x_scales, out, out_dtype)
+    if out is not None:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        out_dtype = out.dtype
+    if isinstance(w, MXFP4Stack):
+        E, M, K = w.num_experts, w.rows, w.cols
+        P = _grouped_rows(x, torch.bfloat16 if x_scales is None else torch.uint8, "x", offsets, E)
+        if x.shape[1] != (K if x_scales is None else K // 2):
+            raise ValueError(f"x has {x.shape[1]} columns, weights expect {K if x_scales is None else K // 2}")
+        if w.codes.device != x.device:
+            raise ValueError("w and rows must be on the same device")
+        if x_scales is not None:
+            _dev(x_scales, torch.uint8, "x_scales")
+            if tuple(x_scales.shape) != (P, K // 32) or x_scales.device != x.device:
+                raise ValueError(f"x_scales must be [{P}, {K // 32}] on {x.device}")
+        y = _grouped_out(out, out_dtype or torch.bfloat16, (P, M), x.device)
+        d = w.desc()
+        N.check("lutmoe_grouped_gemm_mxfp4", N.lib().lutmoe_grouped_gemm_mxfp4(
+            ctypes.byref(d), x.data_ptr(), N.DTYPE_BF16 if x_scales is None else N.DTYPE_MXFP4,
+            None if x_scales is None else x_scales.data_ptr(), offsets.data_ptr(), P, y.data_ptr(),
+            _GROUPED_DT[y.dtype], int(out is None), _stream()))
+        return y
+    if not isinstance(w, torch.Tensor):
+        raise TypeError("w must be a tensor [E, M, K] or an MXFP4Stack")
+    if x_scales is not None:
+        raise ValueError("x_scales given, but w is not an MXFP4Stack")
+    if w.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"w must be bfloat16 or float16, got {w.dtype}")
+    E, M, K = _grouped_weights(w, w.dtype, x.device)
+    P = _grouped_rows(x, w.dtype, "x", offsets, E)
+    if x.shape[1] != K:
+        raise ValueError(f"x has {x.shape[1]} columns, weights expect {K}")
+    y = _grouped_out(out, out_dtype or x.dtype, (P, M), x.device)
+    N.check("lutmoe_grouped_gemm", N.lib().lutmoe_grouped_gemm(
+        x.data_ptr(), _GROUPED_DT[x.dtype], w.data_ptr(), offsets.data_ptr(), E, P, M, K, y.data_ptr(),
+        _GROUPED_DT[y.dtype], int(out is None), _stream()))
+    return y
+
+
+def grouped_gemm_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The gradient of ``grouped_gemm``'s rows: dx[p] = dy[p] . W[e] for the rows p of group e.
+    dy [P, M], w [E, M, K] in bf16 or fp16; rows of no group as in ``grouped_gemm``."""
+    if isinstance(dy, torch.Tensor) and dy.is_cuda and not _here(dy):
+        with torch.cuda.device(dy.device):
+            return grouped_gemm_dgrad(dy, w, offsets, out, out_dtype)
+    if dy.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"dy must be bfloat16 or float16, got {dy.dtype}")
+    E, M, K = _grouped_weights(w, dy.dtype, dy.device)
+    P = _grouped_rows(dy, dy.dtype, "dy", offsets, E)
+    if dy.shape[1] != M:
+        raise ValueError(f"dy has {dy.shape[1]} columns, weights have {M} rows")
+    dx = _grouped_out(out, out_dtype or (dy.dtype if out is None else out.dtype), (P, K), dy.device)
+    N.check("lutmoe_grouped_gemm_dgrad", N.lib().lutmoe_grouped_gemm_dgrad(
+        dy.data_ptr(), _GROUPED_DT[dy.dtype], w.data_ptr(), offsets.data_ptr(), E, P, M, K, dx.data_ptr(),
+        _GROUPED_DT[dx.dtype], int(out is None), _stream()))
+    return dx
+
+
+def grouped_gemm_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The gradient of ``grouped_gemm``'s matrices: dW[e] = sum of dy[p]^T x[p] over the rows p
+    of group e (zeros for an empty one), [E, M, K].  dy [P, M], x [P, K] in bf16 or fp16."""
+    if isinstance(dy, torch.Tensor) and dy.is_cuda and not _here(dy):
+        with torch.cuda.device(dy.device):
+            return grouped_gemm_wgrad(dy, x, offsets, out, out_dtype)
+    if dy.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"dy must be bfloat16 or float16, got {dy.dtype}")
+    E = offsets.numel() - 1 if isinstance(offsets, torch.Tensor) else 0
+    if E < 1:
+        raise ValueError("offsets must hold one more value than there are experts")
+    P = _grouped_rows(dy, dy.dtype, "dy", offsets, E)
+    _dev(x, dy.dtype, "x")
+    if x.dim() != 2 or x.shape[0] != P or x.device != dy.device:
+        raise ValueError(f"x must be [{P}, K] on {dy.device}")
+    M, K = dy.shape[1], x.shape[1]
+    dw = _grouped_out(out, out_dtype or (dy.dtype if out is None else out.dtype), (E, M, K), dy.device)
+    N.check("lutmoe_grouped_gemm_wgrad", N.lib().lutmoe_grouped_gemm_wgrad(
+        dy.data_ptr(), _GROUPED_DT[dy.dtype], x.data_ptr(), offsets.data_ptr(), E, P, M, K, dw.data_ptr(),
+        _GROUPED_DT[dw.dtype], _stream()))
+    return dw
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets):
+        ctx.save_for_backward(x, w, offsets)
+        return grouped_gemm(x, w, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        dy = dy.contiguous()   # (a sum's gradient is one value, expanded)
+        dx = grouped_gemm_dgrad(dy, w, offsets) if ctx.needs_input_grad[0] else None
+        dw = grouped_gemm_wgrad(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """``grouped_gemm`` of dense matrices with its backward pass: gradients of x (zero in rows
+    of no group) and of w (zero for an expert without rows), both in their dtype from fp32
+    sums.  ``offsets`` must keep its values until the backward pass has run."""
+    return _GroupedLinear.apply(x, w, offsets)
+
+
 # --------------------------------------------------------------- MoE layer
 
 PATH_AUTO, PATH_GEMV, PATH_MFMA = 0, 1, 2
@@ -333,6 +492,28 @@ def bl4_encode(weight: torch.Tensor, n_iter: int = 50) -> Tuple[torch.Tensor, to
                                                            codes.data_ptr(), tables.data_ptr(),
                                                            _stream()))
     return codes, tables
+
+
+def mxfp4_encode(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """MXFP4 encoder on the GPU, for weights and activations.  weight bf16, fp16 or fp32 [..., K],
+    K % 32 == 0.  Returns (codes uint8 [..., K/2], scales uint8 [..., K/32]): blocks of 32 along
+    the last axis, scale 2^(floor(log2(max)) - 2), elements rounded to nearest (ties to the
+    even code), past 6 scales to 6; a block with an infinity or NaN becomes NaN."""
+    if isinstance(weight, torch.Tensor) and weight.is_cuda and not _here(weight):
+        with torch.cuda.device(weight.device):
+            return mxfp4_encode(weight)
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in _GROUPED_DT:
+        raise TypeError("weight must be a bfloat16, float16 or float32 tensor")
+    _dev(weight, weight.dtype, "weight")
+    if weight.dim() < 1 or weight.shape[-1] % 32 or weight.shape[-1] == 0:
+        raise ValueError("K must be a multiple of 32")
+    lead, K = tuple(weight.shape[:-1]), weight.shape[-1]
+    codes = torch.empty(lead + (K // 2,), dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(lead + (K // 32,), dtype=torch.uint8, device=weight.device)
+    N.check("lutmoe_mxfp4_encode", N.lib().lutmoe_mxfp4_encode(weight.data_ptr(), _GROUPED_DT[weight.dtype],
+                                                               weight.numel() // 32, codes.data_ptr(),
+                                                               scales.data_ptr(), _stream()))
+    return codes, scales
 
 
 def ref_encode(weight: torch.Tensor, codebook: torch.Tensor, block_size: int = 128

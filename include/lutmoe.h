@@ -27,6 +27,11 @@
  *          w_{n+24}; b2: nibble n bit q = bit 2 of w_{n+8q} (b >= 3); b3:
  *          bit 3 likewise (b = 4) -- 4b bytes per group, M*K*b/8 per expert
  *          (lutmoe_nested_group_planes converts).  Tables bf16 [M][K/64][2^b].
+ *   MXFP4: codes uint8 [E][M][K/2] (4-bit E2M1 elements 0, .5, 1, 1.5, 2, 3, 4,
+ *          6 and, with bit 3, their negatives; even element in the low nibble),
+ *          scales uint8 [E][M][K/32], one per 32 consecutive elements of a
+ *          row: byte b stands for 2^(b - 127), 255 for NaN.  K % 32 == 0.
+ *          Taken by lutmoe_dequant, lutmoe_gemv and the grouped products.
  */
 #ifndef LUTMOE_H
 #define LUTMOE_H
@@ -50,9 +55,12 @@ extern "C" {
 #define LUTMOE_FMT_REF        0
 #define LUTMOE_FMT_BL4        1
 #define LUTMOE_FMT_NESTED     2
+#define LUTMOE_FMT_MXFP4      3
 
 #define LUTMOE_DTYPE_BF16     0
 #define LUTMOE_DTYPE_F32      1
+#define LUTMOE_DTYPE_F16      2   /* encoder input and grouped products */
+#define LUTMOE_DTYPE_MXFP4    3   /* rows of the grouped products       */
 
 /* One stack of per-expert LUT-quantised matrices W[e] of shape [rows, cols]
  * (rows = output features, cols = K = input features). */
@@ -61,11 +69,12 @@ typedef struct lutmoe_weights {
     int32_t num_experts;       /* E                                              */
     int32_t rows;              /* M                                              */
     int32_t cols;              /* K                                              */
-    const void* codes;         /* REF/BL4: device base of [E] code arrays.
+    const void* codes;         /* REF/BL4/MXFP4: device base of [E] code arrays.
                                   NL: device array of E pointers (uint8_t*) to
                                   each expert's grouped codes (M*K*b/8 bytes).   */
     const void* tables;        /* REF: bf16 absmax [E][absmax_per_expert].
                                   BL4: bf16 tables [E][M][K/64][16].
+                                  MXFP4: uint8 scales [E][M][K/32].
                                   NL: device array of E pointers (uint16_t*) to
                                   each expert's bf16 table [M][K/64][2^b].       */
     const void* codebook;      /* REF: bf16[256] codebook(s); else NULL.         */
@@ -220,7 +229,7 @@ int lutmoe_gemv(const lutmoe_weights* w, int expert, const void* x_dev, int T,
  * LUTMOE_DTYPE_F32 (BL4 and REF weights; fp32 x: each weight widened to fp32
  * and multiplied by an fp32 FMA, REF in lut_gemv's (x * cb) * absmax order --
  * the reference's CPU dequant + F.linear on fp32 inputs,
- * vllm_lut/quantizer.py:449-477).  NestedLUT takes bf16 x only
+ * vllm_lut/quantizer.py:449-477).  NestedLUT and MXFP4 take bf16 x only
  * (LUTMOE_EUNSUPPORTED). */
 int lutmoe_gemv_ex(const lutmoe_weights* w, int expert, const void* x_dev, int x_dtype, int T,
                    void* y_dev, int y_dtype, void* stream);
@@ -337,6 +346,46 @@ int lutmoe_moe_forward_logits_ex(const lutmoe_moe_desc* d, const void* x_dev, co
                                  void* workspace_dev, size_t workspace_bytes, int force_path, int stages,
                                  void* stream);
 
+/* ---- grouped products ----------------------------------------------------- */
+
+/* Products of rows sorted by expert (no counterpart in the reference, whose
+ * layers multiply one expert after another).  Group e is the rows
+ * [offsets[e], offsets[e+1]) of the P rows, in the order lutmoe_permute gives:
+ * offsets_dev int32 [E+1], offsets[0] taken as 0, not decreasing, at most P
+ * (values outside [0, P] are clamped; with decreasing ones the results are
+ * unspecified, and no access leaves the arrays).  A group may be empty; rows
+ * behind the last group belong to none.  fp32 accumulation, one rounding.
+ *
+ * Common rules: E <= 4096; P >= 0; 1 <= M, K <= 2^20; x, dy and the matrices
+ * 16-byte aligned, results aligned to their elements (16 bytes are faster);
+ * results do not depend on scheduling.  zero_rest != 0 sets the result's rows of no group to zero; else
+ * they are left as they were.  The calls need no workspace, allocate nothing and
+ * can be captured. */
+
+/* Dense matrices: y[p][0..M) = x[p] . W[e]^T for the rows p of group e.
+ * x [P][K], W [E][M][K], both of dtype LUTMOE_DTYPE_BF16 or LUTMOE_DTYPE_F16;
+ * y [P][M] of that dtype or LUTMOE_DTYPE_F32.  M % 8 == 0 and K % 8 == 0. */
+int lutmoe_grouped_gemm(const void* x_dev, int dtype, const void* w_dev, const int32_t* offsets_dev, int E, int P,
+                        int M, int K, void* y_dev, int y_dtype, int zero_rest, void* stream);
+
+/* The gradients of lutmoe_grouped_gemm.  dgrad: dx[p][0..K) = dy[p] . W[e].
+ * wgrad: dW[e] = sum over the rows p of group e of dy[p]^T x[p], [E][M][K]
+ * (zeros for an empty group).  dy [P][M], x, W of `dtype`; the results of that
+ * dtype or fp32. */
+int lutmoe_grouped_gemm_dgrad(const void* dy_dev, int dtype, const void* w_dev, const int32_t* offsets_dev, int E,
+                              int P, int M, int K, void* dx_dev, int dx_dtype, int zero_rest, void* stream);
+int lutmoe_grouped_gemm_wgrad(const void* dy_dev, int dtype, const void* x_dev, const int32_t* offsets_dev, int E,
+                              int P, int M, int K, void* dw_dev, int dw_dtype, void* stream);
+
+/* MXFP4 matrices: y[p] = x[p] . W[e]^T, w->format == LUTMOE_FMT_MXFP4.  x_dtype
+ * LUTMOE_DTYPE_BF16: x [P][K], x_scales_dev NULL, the weights widened to bf16
+ * (exact).  LUTMOE_DTYPE_MXFP4: x codes [P][K/2], x_scales_dev [P][K/32] as
+ * lutmoe_mxfp4_encode gives them, multiplied by the scaled MFMA.  y [P][M] bf16
+ * or fp32, any M. */
+int lutmoe_grouped_gemm_mxfp4(const lutmoe_weights* w, const void* x_dev, int x_dtype, const uint8_t* x_scales_dev,
+                              const int32_t* offsets_dev, int P, void* y_dev, int y_dtype, int zero_rest,
+                              void* stream);
+
 /* ---- measurement ---------------------------------------------------------- */
 
 /* The HBM floor of the one-token BL4 layer (no counterpart in the reference;
@@ -357,6 +406,16 @@ int lutmoe_decode_stream_probe(const lutmoe_moe_desc* d, const int32_t* ids_dev,
  * packed codes [nblocks*32] and fp16 tables [nblocks*16]. */
 int lutmoe_bl4_encode(const float* w_dev, int64_t nblocks, int n_iter, uint8_t* codes_dev,
                       uint16_t* tables_f16_dev, void* stream);
+
+/* MXFP4 encoder: x [nblocks*32] of x_dtype (bf16, fp16 or fp32; 16-byte
+ * aligned) -> packed codes [nblocks*16] (16-byte aligned) and scale bytes
+ * [nblocks].  The block's scale is 2^(floor(log2(max |x|)) - 2) (not below
+ * 2^-127; byte 0 for a block of zeros), an element x / scale rounded to the
+ * nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (ties to the even code; past 6 to 6; the
+ * sign is kept, also of zero).  A block that holds an infinity or NaN: scale byte
+ * 255 (NaN), codes 0.  No counterpart in the reference. */
+int lutmoe_mxfp4_encode(const void* x_dev, int x_dtype, int64_t nblocks, uint8_t* codes_dev, uint8_t* scales_dev,
+                        void* stream);
 
 /* REF encoder, replacing encode_blocklut_kernel / launch_encode
  * (vllm_lut/fast_encode.py:22-72, 80-99): bf16 weights [n] and an fp32[256]
