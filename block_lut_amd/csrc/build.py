@@ -19,7 +19,7 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "liblutmoe.so")
 SOURCES = ["api.cpp", "dequant.hip", "gemv.hip", "decode.hip", "route.hip", "gemm.hip",
            "encode.hip", "noalloc.hip", "dense.hip", "stream.hip",
-           "mxfp4.hip", "grouped.hip"]
+           "mxfp4.hip", "grouped.hip", "grouped_tile.hip"]
 ARCH = "gfx950"
 
 

@@ -123,6 +123,7 @@ __global__ __launch_bounds__(256) void simple_kernel(GroupedArgs g) {
 namespace lutmoe_host {
 
 int launch_grouped(const GroupedArgs& g, hipStream_t s) {
+    if (!g.w_scales || g.x_scales) return launch_grouped_tile(g, s);
     const int C = g.op == kGroupedFwd ? g.M : g.K;
     const int64_t rows = g.op == kGroupedWgrad ? (g.M + kB - 1) / kB : g.P / kB + (g.P < g.E + 1 ? g.P : g.E + 1);
     const dim3 grid((uint32_t)rows, (C + kB - 1) / kB, g.op == kGroupedWgrad ? g.E : 1), block(256);

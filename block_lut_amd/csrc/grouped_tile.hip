@@ -1,0 +1,462 @@
+// Products of rows sorted by expert, tiles: C[r][c] = sum_k A(r, k) B(c, k) with
+//   forward  r a group's rows, c the rows of W[e], k columns: both operands k-contiguous
+//   dgrad    r a group's rows, c columns of W[e], k rows of W[e]: W transposed on its way
+//   wgrad    r rows of dW[e], c its columns, k the group's rows: both transposed
+// on MFMA (16 x 16 x 32, 16-bit operands; forward with both operands in MXFP4: the scaled
+// 16 x 16 x 128, four times the columns in the same bytes).
+//
+// A CTA is 8 waves (2 along r x 4 along c, a wave 128 x 64) on a tile of up to 256 x 256.
+// K goes in steps of 64 bytes a row (32 columns, MXFP4: 128) through a ring of stages of 32 KB,
+// filled by 16-byte LDS DMA; a step's fragments are read while the one before is multiplied.
+// Layouts of a stage (all reads without bank conflicts):
+//   k-contiguous  64-byte rows, 16-byte chunk q of row r at q ^ (r / 4 % 4) (c: q ^ (r / 16 % 4))
+//   transposed    512-byte rows of 256 columns, read by the transposing LDS read
+//                 (ds_read_b64_tr_b16: 4 rows x 16 columns -> 4 elements of a column a lane)
+// Fragment f of the c operand takes the columns 16 (i / 4) + 4 f + i % 4 (i its row), so that a
+// lane's accumulators are 16 consecutive results of one row: whole 16-byte stores.
+// Ragged groups: a group's last tile computes 64, 128 or 192 rows where that is enough (the
+// two waves of a column block take alternate 16-row fragments).
+#include "common.h"
+#include "kernels.h"
+#include "lut_core.h"
+
+using namespace lutmoe;
+using lutmoe_host::GroupedArgs;
+
+namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
+typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8_t;
+
+constexpr int kTile = 256;
+constexpr int kOperand = 16384;   // stage bytes of an operand
+constexpr int kF4 = 4;            // (kT) LUTMOE_DTYPE_*; both operands MXFP4
+
+template <int kT, int kSD>
+struct Ring {
+    static constexpr int kStage = 2 * kOperand + 2048 * kSD;   // MXFP4: 512 rows' scales, kSD dwords each
+    static constexpr int kStages = kT == kF4 ? 4 : 5;
+    static constexpr int kStep = kT == kF4 ? 128 : 32;         // columns
+};
+
+__device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t m0) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t m0) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+}
+template <int kAfter>
+__device__ __forceinline__ void wait_barrier() {
+    static_assert(kAfter >= 0 && kAfter <= 63, "vmcnt range");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kAfter) : "memory");
+}
+
+typedef __attribute__((address_space(3))) const u32x4_t* lds_quad_t;
+typedef __attribute__((address_space(3))) s16x4_t* lds_tr_t;
+typedef __attribute__((address_space(3))) const uint8_t* lds_byte_t;
+__device__ __forceinline__ u32x4_t lds_quad(uint32_t a) { return *(lds_quad_t)a; }
+// 8 elements k of one column: two transposing reads 4 rows (2 KB) apart
+__device__ __forceinline__ u32x4_t lds_tr(uint32_t a) {
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t)a);
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t)(a + 2048u));
+    const u32x2_t l = __builtin_bit_cast(u32x2_t, lo), h = __builtin_bit_cast(u32x2_t, hi);
+    return u32x4_t{l[0], l[1], h[0], h[1]};
+}
+
+// Group e's rows, clamped into [0, P] (the first starts at row 0); e = E: the rows behind.
+__device__ __forceinline__ void group_rows(const GroupedArgs& g, int e, int& p0, int& n) {
+    const int a = e <= 0 || !g.offsets ? 0 : min(max(g.offsets[min(e, g.E)], 0), g.P);
+    const int b = e >= g.E || !g.offsets ? g.P : min(max(g.offsets[e + 1], 0), g.P);
+    p0 = a;
+    n = e > g.E ? 0 : max(b - a, 0);
+}
+
+struct TileAt {
+    int e, p0, n;   // group (E: the rows behind), its first row, rows
+    int r0, c0;     // first row and column of the tile
+};
+
+__device__ __forceinline__ int wave_scan(int v) {   // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, kWave);
+        v += lane >= o ? u : 0;
+    }
+    return v;
+}
+
+// The tile of a CTA: each eighth of the tiles runs on one XCD (a CTA's index modulo 8), group
+// by group; in a group up to 8 row tiles go along with a column tile.  Every wave
+// finds it by itself: tiles of 64 groups at a time summed up across its lanes.
+template <int kOp>
+__device__ __forceinline__ bool find_tile(const GroupedArgs& g, int nct, TileAt& t) {
+    const int lane = threadIdx.x & 63, b = blockIdx.x;
+    if constexpr (kOp == kGroupedWgrad) {
+        const int nrt = (g.M + kTile - 1) / kTile, each = nrt * nct, total = g.E * each, per = (total + 7) / 8;
+        const int i = (b & 7) * per + (b >> 3);
+        if ((b >> 3) >= per || i >= total) return false;
+        t.e = i / each;
+        const int in = i - t.e * each;
+        t.r0 = in / nct * kTile;
+        t.c0 = (in - in / nct * nct) * kTile;
+        group_rows(g, t.e, t.p0, t.n);
+        t.p0 = __builtin_amdgcn_readfirstlane(t.p0);
+        t.n = __builtin_amdgcn_readfirstlane(t.n);
+        return true;
+    }
+    const int groups = g.E + (g.zero_rest ? 1 : 0);
+    int total = 0;
+    for (int e0 = 0; e0 < groups; e0 += 64) {
+        int p0, n;
+        group_rows(g, e0 + lane, p0, n);
+        if (e0 + lane >= groups) n = 0;
+        total += __builtin_amdgcn_readlane(wave_scan((n + kTile - 1) / kTile), 63);
+    }
+    total *= nct;
+    const int per = (total + 7) / 8, i = (b & 7) * per + (b >> 3);
+    if ((b >> 3) >= per || i >= total) return false;
+    int before = 0;
+    for (int e0 = 0; e0 < groups; e0 += 64) {
+        int p0, n;
+        group_rows(g, e0 + lane, p0, n);
+        if (e0 + lane >= groups) n = 0;
+        const int mine = (n + kTile - 1) / kTile, upto = wave_scan(mine);
+        const uint64_t m = __ballot(i < before + upto * nct);
+        if (m) {
+            const int l = __builtin_ctzll(m);
+            t.e = e0 + l;
+            t.p0 = __builtin_amdgcn_readlane(p0, l);
+            t.n = __builtin_amdgcn_readlane(n, l);
+            const int mt = __builtin_amdgcn_readlane(mine, l);
+            const int in = i - before - (__builtin_amdgcn_readlane(upto, l) - mt) * nct;
+            const int grp = in / (8 * nct), size = min(8, mt - 8 * grp), rem = in - grp * 8 * nct;
+            const int ct = rem / size;
+            t.r0 = (8 * grp + rem - ct * size) * kTile;
+            t.c0 = ct * kTile;
+            // (decreasing offsets can count more tiles than an int holds)
+            return (uint32_t)t.r0 < (uint32_t)t.n && (uint32_t)t.c0 < (uint32_t)nct * kTile;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63) * nct;
+    }
+    return false;
+}
+
+template <int kT>
+__device__ __forceinline__ f32x4_t mma(u32x4_t c, u32x4_t r, f32x4_t acc, int sc, int sr) {
+    if constexpr (kT == kF4) {
+        const i32x8_t a = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+        const i32x8_t b = {(int)r[0], (int)r[1], (int)r[2], (int)r[3], 0, 0, 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, sc, 0, sr);
+    } else if constexpr (kT == LUTMOE_DTYPE_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, c), __builtin_bit_cast(f16x8_t, r), acc, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, c), __builtin_bit_cast(bf16x8_t, r), acc, 0, 0, 0);
+    }
+}
+
+// 16 results of a row from its column c: whole where the row is aligned, else one by one.
+__device__ __forceinline__ void store16(const GroupedArgs& g, int64_t row, int c, int C, const f32x4_t (&v)[4]) {
+    if (c >= C) return;
+    const int64_t o = row * C + c;
+    if (g.out_dtype == LUTMOE_DTYPE_F32) {
+        float* p = (float*)g.out + o;
+        if (g.out_vec) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + 4 * q < C) *(f32x4_t*)(p + 4 * q) = v[q];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (c + q < C) p[q] = v[q >> 2][q & 3];
+        }
+        return;
+    }
+    uint32_t u[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const float a = v[q >> 1][2 * (q & 1)], b = v[q >> 1][2 * (q & 1) + 1];
+        u[q] = g.out_dtype == LUTMOE_DTYPE_F16 ? f32_to_f16(a) | f32_to_f16(b) << 16 : f32x2_to_bf16x2(a, b);
+    }
+    uint16_t* p = (uint16_t*)g.out + o;
+    if (g.out_vec) {
+        *(u32x4_t*)p = u32x4_t{u[0], u[1], u[2], u[3]};
+        if (c + 8 < C) *(u32x4_t*)(p + 8) = u32x4_t{u[4], u[5], u[6], u[7]};
+    } else {
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if (c + q < C) p[q] = (uint16_t)(u[q >> 1] >> (16 * (q & 1)));
+    }
+}
+
+// MF: 16-row fragments of a wave (the tile has 32 MF rows).
+template <int kOp, int kT, int kSD, int MF>
+__device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, uint8_t* ring) {
+    using Rg = Ring<kT, kSD>;
+    constexpr int S = Rg::kStages, kStep = Rg::kStep, kChunk = kStep / 4;   // columns of a 16-byte chunk
+    constexpr bool kRtr = kOp == kGroupedWgrad, kCtr = kOp != kGroupedFwd;
+    constexpr int LR = kRtr ? 4 : MF / 2;   // DMAs of a wave that loads rows (the others: 4)
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int C = kOp == kGroupedFwd ? g.M : g.K;
+    const int nrows = min(32 * MF, (kRtr ? g.M : t.n) - t.r0);   // valid rows of the tile
+    const int Kt = t.e >= g.E ? 0 : kOp == kGroupedFwd ? g.K : kOp == kGroupedDgrad ? g.M : t.n;
+    const int nk = (Kt + kStep - 1) / kStep, rem = Kt - (nk - 1) * kStep;   // columns of the last step
+
+    // ---- loader: waves 0 .. 3 the r operand, 4 .. 7 the c operand
+    const bool is_r = wv < 4;
+    const int lw = wv & 3, row_bytes_k = kT == kF4 ? g.K / 2 : 2 * (kOp == kGroupedDgrad ? g.M : g.K);
+    const uint8_t* base;
+    int64_t advance = 64;
+    uint32_t off[4];
+    if ((is_r && !kRtr) || (!is_r && !kCtr)) {
+        const int valid = is_r ? nrows : min(kTile, C - t.c0);
+        base = is_r ? (const uint8_t*)g.x + (int64_t)(t.p0 + t.r0) * row_bytes_k
+                    : (const uint8_t*)g.w + ((int64_t)t.e * g.M + t.c0) * row_bytes_k;
+        const int nl = is_r ? LR : 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = min(16 * (nl * lw + j) + (lane >> 2), valid - 1);
+            const int chunk = (lane & 3) ^ (is_r ? lane >> 4 : j);
+            off[j] = (uint32_t)row * (uint32_t)row_bytes_k + 16u * (uint32_t)chunk;
+        }
+    } else {
+        // 512-byte rows of 256 columns: two rows a DMA
+        const int cols = is_r ? g.M : C, first = is_r ? t.r0 : t.c0, ld = 2 * cols;
+        base = is_r ? (const uint8_t*)g.x + (int64_t)t.p0 * ld
+                    : (const uint8_t*)g.w + (kOp == kGroupedDgrad ? (int64_t)t.e * g.M : (int64_t)t.p0) * ld;
+        advance = (int64_t)kStep * ld;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = 2 * (4 * lw + j) + (lane >> 5);
+            const int h = is_r ? ((row & 3) << 1) | (row & 8) : (row & 1) | ((row & 2) << 2);
+            const int chunk = min(first / 8 + ((lane & 31) ^ h), cols / 8 - 1);
+            off[j] = (uint32_t)row * (uint32_t)ld + 16u * (uint32_t)chunk;
+        }
+    }
+    // MXFP4: the scale bytes of row `lane` of the wave's 64: the dword that holds the step's four
+    // (kSD 2: the two, at any alignment), `so` from the wave's aligned base
+    const uint8_t* sbase = nullptr;
+    uint32_t so = 0;
+    int64_t slast = 0;
+    if constexpr (kSD > 0) {
+        const int kb = g.K / 32, valid = is_r ? nrows : min(kTile, C - t.c0);
+        const uint8_t* s0 = is_r ? (const uint8_t*)g.x_scales + (int64_t)(t.p0 + t.r0) * kb
+                                 : (const uint8_t*)g.w_scales + ((int64_t)t.e * g.M + t.c0) * kb;
+        const uint8_t* end = is_r ? (const uint8_t*)g.x_scales + (int64_t)g.P * kb
+                                  : (const uint8_t*)g.w_scales + (int64_t)g.E * g.M * kb;
+        const uint32_t d = kSD == 2 ? (uint32_t)((uintptr_t)s0 & 3) : 0u;
+        sbase = s0 - d;
+        so = (d + (uint32_t)min(64 * lw + lane, valid - 1) * (uint32_t)kb) & ~3u;
+        slast = (int64_t)((((uintptr_t)end - 1) & ~(uintptr_t)3) - (uintptr_t)sbase);
+    }
+    const uint32_t l_ring = lds_addr(ring);
+    // the last step's offsets, where it is short: what lies past the end is read from the
+    // step's first chunk (row) instead
+    auto tail_off = [&](int j) __attribute__((always_inline)) {
+        if ((is_r && !kRtr) || (!is_r && !kCtr)) {
+            const int chunk = (lane & 3) ^ (is_r ? lane >> 4 : j);
+            return off[j] - (chunk * kChunk >= rem ? 16u * (uint32_t)chunk : 0u);
+        }
+        const int row = 2 * (4 * lw + j) + (lane >> 5);
+        return off[j] - (row >= rem ? (uint32_t)row * (uint32_t)(2 * (is_r ? g.M : C)) : 0u);
+    };
+    auto issue = [&](int k, uint32_t slot) __attribute__((always_inline)) {
+        const uint8_t* b = base + (int64_t)k * advance;
+        const uint32_t l0 = l_ring + slot + (is_r ? (uint32_t)(LR * lw) * 1024u : (uint32_t)kOperand + (uint32_t)lw * 4096u);
+        if (kSD != 1 && k == nk - 1 && rem < kStep) {   // (kSD 1: whole steps)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (!is_r || j < LR) dma16(tail_off(j), b, l0 + 1024u * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (!is_r || j < LR) dma16(off[j], b, l0 + 1024u * j);
+        }
+        if constexpr (kSD > 0) {
+            const uint32_t ls = l_ring + slot + 2 * kOperand + (is_r ? 0u : 1024u) + 256u * (uint32_t)lw;
+            dma4(so, sbase + 4 * (int64_t)k, ls);
+            if constexpr (kSD == 2) {
+                const int64_t last = slast - 4 * (int64_t)k;   // (the last dword of the array)
+                dma4((uint32_t)min((int64_t)so + 4, last), sbase + 4 * (int64_t)k, ls + 2048u);
+            }
+        }
+    };
+
+    // ---- compute side
+    const int i = lane & 15, gq = lane >> 4, wm = wv >> 2, wn = wv & 3;
+    const int iq = i >> 2, ib = i & 3;
+    uint32_t ar, ac;
+    if constexpr (kRtr) ar = (uint32_t)((8 * gq + iq) * 512 + 16 * ((2 * wm + (ib >> 1)) ^ ((iq << 1) | ((gq & 1) << 3))) + 8 * (ib & 1));
+    else ar = (uint32_t)((16 * wm + i) * 64 + 16 * (gq ^ iq));
+    if constexpr (kCtr) ac = (uint32_t)((8 * gq + iq) * 512 + 16 * ((8 * wn + 2 * ib) ^ ((iq & 1) | ((iq >> 1) << 3))));
+    else ac = (uint32_t)((64 * wn + 16 * iq + ib) * 64 + 16 * (gq ^ iq));
+    ar += l_ring;
+    ac += l_ring + kOperand;
+    uint32_t asr = 0, asc = 0;   // MXFP4: scale byte addresses
+    if constexpr (kSD > 0) {
+        auto at = [&](const void* s, int64_t row0, int row) __attribute__((always_inline)) {
+            uint32_t q = (uint32_t)gq;
+            if constexpr (kSD == 2) q += ((uint32_t)((uintptr_t)s & 3) + (uint32_t)((row0 + row) & 3) * (uint32_t)((g.K / 32) & 3)) & 3u;
+            return (uint32_t)(row * 4) + (q >> 2) * 2048u + (q & 3u);
+        };
+        asr = l_ring + 2 * kOperand + at(g.x_scales, t.p0 + t.r0, 16 * wm + i);
+        asc = l_ring + 2 * kOperand + 1024 + at(g.w_scales, (int64_t)t.e * g.M + t.c0, 64 * wn + 16 * iq + ib);
+    }
+    // A step's c fragments are read while the one before is multiplied, an r fragment right
+    // after the last product of the one that it replaces: a read has most of a step to arrive
+    struct ColFrags {
+        u32x4_t v[4];
+        int s[4];
+    };
+    ColFrags fc[2];
+    u32x4_t fr[MF];
+    int sr[MF];
+    auto read_c = [&](uint32_t slot, ColFrags& F, int f) __attribute__((always_inline)) {
+        if constexpr (kCtr) F.v[f] = lds_tr(((ac + slot) ^ (uint32_t)(16 * (f >> 1))) + 8 * (f & 1));
+        else F.v[f] = lds_quad(ac + slot + 256 * f);
+        F.s[f] = 0;
+        if constexpr (kSD > 0) F.s[f] = *(lds_byte_t)(asc + slot + 16 * f);
+    };
+    auto read_r = [&](uint32_t slot, int m) __attribute__((always_inline)) {
+        if constexpr (kRtr) fr[m] = lds_tr(((ar + slot) ^ (uint32_t)(64 * (m & 3))) + 256 * (m >> 2));
+        else fr[m] = lds_quad(ar + slot + 2048 * m);
+        sr[m] = 0;
+        if constexpr (kSD > 0) sr[m] = *(lds_byte_t)(asr + slot + 128 * m);
+    };
+    // columns past the end of the last step: zero in both operands (what was loaded
+    // there belongs to something else)
+    auto mask = [&](ColFrags& F) __attribute__((always_inline)) {
+        uint32_t keep[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const int k = kRtr ? 8 * gq + 2 * d : kChunk * gq;   // (wgrad: single rows end, else whole chunks)
+            keep[d] = !kRtr ? (k < rem ? 0xffffffffu : 0u) : k + 1 < rem ? 0xffffffffu : k < rem ? 0xffffu : 0u;
+        }
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) F.v[f][d] &= keep[d];
+            if constexpr (kSD > 0) F.s[f] &= keep[0];
+        }
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) fr[m][d] &= keep[d];
+            if constexpr (kSD > 0) sr[m] &= keep[0];
+        }
+    };
+    f32x4_t acc[MF][4];
+#pragma unroll
+    for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[m][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    // at most `after` stages issued later than the one needed may be in flight
+    auto wait_stage = [&](int after) __attribute__((always_inline)) {
+        if (is_r) {
+            constexpr int L = LR + kSD;
+            if (after >= S - 3) wait_barrier<(S - 3) * L>();
+            else if (after == 1) wait_barrier<L>();
+            else wait_barrier<0>();
+        } else {
+            constexpr int L = 4 + kSD;
+            if (after >= S - 3) wait_barrier<(S - 3) * L>();
+            else if (after == 1) wait_barrier<L>();
+            else wait_barrier<0>();
+        }
+    };
+    if (nk > 0) {
+        for (int k = 0; k < min(S - 1, nk); ++k) issue(k, (uint32_t)k * Rg::kStage);
+        wait_stage(min(S - 2, nk - 1));   // stage 0 has landed (the count of S - 3 stages waits for one more)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) read_c(0, fc[0], f);
+#pragma unroll
+        for (int m = 0; m < MF; ++m) read_r(0, m);
+        // slots of the steps k - 1 (refilled: every wave has multiplied it when step k's
+        // barrier is behind it) and k + 1
+        uint32_t prev = (uint32_t)(S - 1) * Rg::kStage, next = Rg::kStage;
+        auto after_slot = [&](uint32_t s) __attribute__((always_inline)) {
+            return s == (uint32_t)(S - 1) * Rg::kStage ? 0u : s + (uint32_t)Rg::kStage;
+        };
+        auto step = [&](ColFrags& F0, ColFrags& F1, int k) __attribute__((always_inline)) {
+            wait_stage(min(S - 3, nk - 2 - k));
+            if (k - 1 + S < nk) issue(k - 1 + S, prev);
+#pragma unroll
+            for (int m = 0; m < MF; ++m) {
+                if (m < 4 && MF >= 4) read_c(next, F1, m);
+                else if (m < 2) { read_c(next, F1, 2 * m); read_c(next, F1, 2 * m + 1); }
+#pragma unroll
+                for (int f = 0; f < 4; ++f) acc[m][f] = mma<kT>(F0.v[f], fr[m], acc[m][f], F0.s[f], sr[m]);
+                read_r(next, m);
+                __builtin_amdgcn_sched_barrier(0);   // (a read hoisted higher takes registers that are not there)
+            }
+            prev = after_slot(prev);
+            next = after_slot(next);
+        };
+        for (int k = 0; k + 1 < nk; k += 2) {
+            step(fc[0], fc[1], k);
+            if (k + 2 < nk) step(fc[1], fc[0], k + 1);
+            else fc[0] = fc[1];
+        }
+        if (kSD != 1 && rem < kStep) mask(fc[0]);
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) acc[m][f] = mma<kT>(fc[0].v[f], fr[m], acc[m][f], fc[0].s[f], sr[m]);
+    }
+    const int64_t row0 = kRtr ? (int64_t)t.e * g.M + t.r0 : t.p0 + t.r0;
+    const int c = t.c0 + 64 * wn + 16 * gq;
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+        const int r = 32 * m + 16 * wm + i;
+        if (r < nrows) store16(g, row0 + r, c, C, acc[m]);
+    }
+}
+
+template <int kOp, int kT, int kSD>
+__global__ __launch_bounds__(512, 2) void tile_kernel(GroupedArgs g, int nct) {
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[Ring<kT, kSD>::kStages * Ring<kT, kSD>::kStage];
+    TileAt t;
+    if (!find_tile<kOp>(g, nct, t)) return;
+    const int rows = (kOp == kGroupedWgrad ? g.M : t.n) - t.r0;
+    if (rows > 192) run_tile<kOp, kT, kSD, 8>(g, t, ring);
+    else if (rows > 128) run_tile<kOp, kT, kSD, 6>(g, t, ring);
+    else if (rows > 64) run_tile<kOp, kT, kSD, 4>(g, t, ring);
+    else run_tile<kOp, kT, kSD, 2>(g, t, ring);
+}
+
+template <int kOp, int kT, int kSD>
+int tile_launch(const GroupedArgs& g, hipStream_t s) {
+    const int C = kOp == kGroupedFwd ? g.M : g.K, nct = (C + kTile - 1) / kTile;
+    // row tiles: a group's last one may be short
+    const int64_t groups = g.E + (g.zero_rest ? 1 : 0);
+    const int64_t rt = kOp == kGroupedWgrad ? (int64_t)g.E * ((g.M + kTile - 1) / kTile)
+                                            : g.P / kTile + (g.P < groups ? g.P : groups);
+    const int64_t ctas = 8 * ((rt * nct + 7) / 8);
+    if (ctas >= (int64_t(1) << 31)) return LUTMOE_EUNSUPPORTED;
+    hipLaunchKernelGGL((tile_kernel<kOp, kT, kSD>), dim3((uint32_t)ctas), dim3(512), 0, s, g, nct);
+    return lutmoe_host::check_launch();
+}
+
+}  // namespace
+
+namespace lutmoe_host {
+
+int launch_grouped_tile(const GroupedArgs& g, hipStream_t s) {
+    const bool f16 = g.x_dtype == LUTMOE_DTYPE_F16;
+    switch (g.op) {
+        case kGroupedFwd:
+            if (g.x_dtype == LUTMOE_DTYPE_MXFP4) {
+                const bool whole = g.K % 128 == 0 && (uintptr_t)g.x_scales % 4 == 0 && (uintptr_t)g.w_scales % 4 == 0;
+                return whole ? tile_launch<kGroupedFwd, kF4, 1>(g, s) : tile_launch<kGroupedFwd, kF4, 2>(g, s);
+            }
+            return f16 ? tile_launch<kGroupedFwd, LUTMOE_DTYPE_F16, 0>(g, s) : tile_launch<kGroupedFwd, LUTMOE_DTYPE_BF16, 0>(g, s);
+        case kGroupedDgrad:
+            return f16 ? tile_launch<kGroupedDgrad, LUTMOE_DTYPE_F16, 0>(g, s) : tile_launch<kGroupedDgrad, LUTMOE_DTYPE_BF16, 0>(g, s);
+        default:
+            return f16 ? tile_launch<kGroupedWgrad, LUTMOE_DTYPE_F16, 0>(g, s) : tile_launch<kGroupedWgrad, LUTMOE_DTYPE_BF16, 0>(g, s);
+    }
+}
+
+}  // namespace lutmoe_host

@@ -195,5 +195,7 @@ struct GroupedArgs {
     int zero_rest;             // forward, dgrad: rows of no group are set to zero (else not written)
 };
 int launch_grouped(const GroupedArgs& g, hipStream_t s);
+// grouped_tile.hip: every product but MXFP4 matrices with bf16 rows
+int launch_grouped_tile(const GroupedArgs& g, hipStream_t s);
 
 }  // namespace lutmoe_host
