@@ -19,7 +19,8 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "liblutmoe.so")
 SOURCES = ["api.cpp", "dequant.hip", "gemv.hip", "decode.hip", "route.hip", "gemm.hip",
            "encode.hip", "noalloc.hip", "dense.hip", "stream.hip",
-           "mxfp4.hip", "grouped.hip", "grouped_tile.hip"]
+           "mxfp4.hip", "grouped.hip", "grouped_tile.hip", "grouped_mx.hip",
+           "grouped_few.hip"]
 ARCH = "gfx950"
 
 

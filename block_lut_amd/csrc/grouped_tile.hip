@@ -16,22 +16,16 @@
 // lane's accumulators are 16 consecutive results of one row: whole 16-byte stores.
 // Ragged groups: a group's last tile computes 64, 128 or 192 rows where that is enough (the
 // two waves of a column block take alternate 16-row fragments).
-#include "common.h"
-#include "kernels.h"
-#include "lut_core.h"
+#include "grouped.h"
 
 using namespace lutmoe;
-using lutmoe_host::GroupedArgs;
 
 namespace {
 
-typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
-typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8_t;
 
 constexpr int kTile = 256;
 constexpr int kOperand = 16384;   // stage bytes of an operand
-constexpr int kF4 = 4;            // (kT) LUTMOE_DTYPE_*; both operands MXFP4
 
 template <int kT, int kSD>
 struct Ring {
@@ -40,22 +34,7 @@ struct Ring {
     static constexpr int kStep = kT == kF4 ? 128 : 32;         // columns
 };
 
-__device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t m0) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
-}
-__device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t m0) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
-}
-template <int kAfter>
-__device__ __forceinline__ void wait_barrier() {
-    static_assert(kAfter >= 0 && kAfter <= 63, "vmcnt range");
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kAfter) : "memory");
-}
-
-typedef __attribute__((address_space(3))) const u32x4_t* lds_quad_t;
 typedef __attribute__((address_space(3))) s16x4_t* lds_tr_t;
-typedef __attribute__((address_space(3))) const uint8_t* lds_byte_t;
-__device__ __forceinline__ u32x4_t lds_quad(uint32_t a) { return *(lds_quad_t)a; }
 // 8 elements k of one column: two transposing reads 4 rows (2 KB) apart
 __device__ __forceinline__ u32x4_t lds_tr(uint32_t a) {
     const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_t)a);
@@ -64,130 +43,19 @@ __device__ __forceinline__ u32x4_t lds_tr(uint32_t a) {
     return u32x4_t{l[0], l[1], h[0], h[1]};
 }
 
-// Group e's rows, clamped into [0, P] (the first starts at row 0); e = E: the rows behind.
-__device__ __forceinline__ void group_rows(const GroupedArgs& g, int e, int& p0, int& n) {
-    const int a = e <= 0 || !g.offsets ? 0 : min(max(g.offsets[min(e, g.E)], 0), g.P);
-    const int b = e >= g.E || !g.offsets ? g.P : min(max(g.offsets[e + 1], 0), g.P);
-    p0 = a;
-    n = e > g.E ? 0 : max(b - a, 0);
-}
-
-struct TileAt {
-    int e, p0, n;   // group (E: the rows behind), its first row, rows
-    int r0, c0;     // first row and column of the tile
-};
-
-__device__ __forceinline__ int wave_scan(int v) {   // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, kWave);
-        v += lane >= o ? u : 0;
-    }
-    return v;
-}
-
-// The tile of a CTA: each eighth of the tiles runs on one XCD (a CTA's index modulo 8), group
-// by group; in a group up to 8 row tiles go along with a column tile.  Every wave
-// finds it by itself: tiles of 64 groups at a time summed up across its lanes.
-template <int kOp>
-__device__ __forceinline__ bool find_tile(const GroupedArgs& g, int nct, TileAt& t) {
-    const int lane = threadIdx.x & 63, b = blockIdx.x;
-    if constexpr (kOp == kGroupedWgrad) {
-        const int nrt = (g.M + kTile - 1) / kTile, each = nrt * nct, total = g.E * each, per = (total + 7) / 8;
-        const int i = (b & 7) * per + (b >> 3);
-        if ((b >> 3) >= per || i >= total) return false;
-        t.e = i / each;
-        const int in = i - t.e * each;
-        t.r0 = in / nct * kTile;
-        t.c0 = (in - in / nct * nct) * kTile;
-        group_rows(g, t.e, t.p0, t.n);
-        t.p0 = __builtin_amdgcn_readfirstlane(t.p0);
-        t.n = __builtin_amdgcn_readfirstlane(t.n);
-        return true;
-    }
-    const int groups = g.E + (g.zero_rest ? 1 : 0);
-    int total = 0;
-    for (int e0 = 0; e0 < groups; e0 += 64) {
-        int p0, n;
-        group_rows(g, e0 + lane, p0, n);
-        if (e0 + lane >= groups) n = 0;
-        total += __builtin_amdgcn_readlane(wave_scan((n + kTile - 1) / kTile), 63);
-    }
-    total *= nct;
-    const int per = (total + 7) / 8, i = (b & 7) * per + (b >> 3);
+// wgrad: every tile of every matrix, in eighths as find_tile's.
+__device__ __forceinline__ bool find_wgrad_tile(const GroupedArgs& g, int nct, TileAt& t) {
+    const int nrt = (g.M + kTile - 1) / kTile, each = nrt * nct, total = g.E * each, per = (total + 7) / 8;
+    const int b = blockIdx.x, i = (b & 7) * per + (b >> 3);
     if ((b >> 3) >= per || i >= total) return false;
-    int before = 0;
-    for (int e0 = 0; e0 < groups; e0 += 64) {
-        int p0, n;
-        group_rows(g, e0 + lane, p0, n);
-        if (e0 + lane >= groups) n = 0;
-        const int mine = (n + kTile - 1) / kTile, upto = wave_scan(mine);
-        const uint64_t m = __ballot(i < before + upto * nct);
-        if (m) {
-            const int l = __builtin_ctzll(m);
-            t.e = e0 + l;
-            t.p0 = __builtin_amdgcn_readlane(p0, l);
-            t.n = __builtin_amdgcn_readlane(n, l);
-            const int mt = __builtin_amdgcn_readlane(mine, l);
-            const int in = i - before - (__builtin_amdgcn_readlane(upto, l) - mt) * nct;
-            const int grp = in / (8 * nct), size = min(8, mt - 8 * grp), rem = in - grp * 8 * nct;
-            const int ct = rem / size;
-            t.r0 = (8 * grp + rem - ct * size) * kTile;
-            t.c0 = ct * kTile;
-            // (decreasing offsets can count more tiles than an int holds)
-            return (uint32_t)t.r0 < (uint32_t)t.n && (uint32_t)t.c0 < (uint32_t)nct * kTile;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63) * nct;
-    }
-    return false;
-}
-
-template <int kT>
-__device__ __forceinline__ f32x4_t mma(u32x4_t c, u32x4_t r, f32x4_t acc, int sc, int sr) {
-    if constexpr (kT == kF4) {
-        const i32x8_t a = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-        const i32x8_t b = {(int)r[0], (int)r[1], (int)r[2], (int)r[3], 0, 0, 0, 0};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, sc, 0, sr);
-    } else if constexpr (kT == LUTMOE_DTYPE_F16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, c), __builtin_bit_cast(f16x8_t, r), acc, 0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, c), __builtin_bit_cast(bf16x8_t, r), acc, 0, 0, 0);
-    }
-}
-
-// 16 results of a row from its column c: whole where the row is aligned, else one by one.
-__device__ __forceinline__ void store16(const GroupedArgs& g, int64_t row, int c, int C, const f32x4_t (&v)[4]) {
-    if (c >= C) return;
-    const int64_t o = row * C + c;
-    if (g.out_dtype == LUTMOE_DTYPE_F32) {
-        float* p = (float*)g.out + o;
-        if (g.out_vec) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (c + 4 * q < C) *(f32x4_t*)(p + 4 * q) = v[q];
-        } else {
-#pragma unroll
-            for (int q = 0; q < 16; ++q)
-                if (c + q < C) p[q] = v[q >> 2][q & 3];
-        }
-        return;
-    }
-    uint32_t u[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const float a = v[q >> 1][2 * (q & 1)], b = v[q >> 1][2 * (q & 1) + 1];
-        u[q] = g.out_dtype == LUTMOE_DTYPE_F16 ? f32_to_f16(a) | f32_to_f16(b) << 16 : f32x2_to_bf16x2(a, b);
-    }
-    uint16_t* p = (uint16_t*)g.out + o;
-    if (g.out_vec) {
-        *(u32x4_t*)p = u32x4_t{u[0], u[1], u[2], u[3]};
-        if (c + 8 < C) *(u32x4_t*)(p + 8) = u32x4_t{u[4], u[5], u[6], u[7]};
-    } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-            if (c + q < C) p[q] = (uint16_t)(u[q >> 1] >> (16 * (q & 1)));
-    }
+    t.e = i / each;
+    const int in = i - t.e * each;
+    t.r0 = in / nct * kTile;
+    t.ct = in - in / nct * nct;
+    group_rows(g, t.e, t.p0, t.n);
+    t.p0 = __builtin_amdgcn_readfirstlane(t.p0);
+    t.n = __builtin_amdgcn_readfirstlane(t.n);
+    return true;
 }
 
 // MF: 16-row fragments of a wave (the tile has 32 MF rows).
@@ -198,7 +66,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     constexpr bool kRtr = kOp == kGroupedWgrad, kCtr = kOp != kGroupedFwd;
     constexpr int LR = kRtr ? 4 : MF / 2;   // DMAs of a wave that loads rows (the others: 4)
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int C = kOp == kGroupedFwd ? g.M : g.K;
+    const int C = kOp == kGroupedFwd ? g.M : g.K, c0 = t.ct * kTile;
     const int nrows = min(32 * MF, (kRtr ? g.M : t.n) - t.r0);   // valid rows of the tile
     const int Kt = t.e >= g.E ? 0 : kOp == kGroupedFwd ? g.K : kOp == kGroupedDgrad ? g.M : t.n;
     const int nk = (Kt + kStep - 1) / kStep, rem = Kt - (nk - 1) * kStep;   // columns of the last step
@@ -210,9 +78,9 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     int64_t advance = 64;
     uint32_t off[4];
     if ((is_r && !kRtr) || (!is_r && !kCtr)) {
-        const int valid = is_r ? nrows : min(kTile, C - t.c0);
+        const int valid = is_r ? nrows : min(kTile, C - c0);
         base = is_r ? (const uint8_t*)g.x + (int64_t)(t.p0 + t.r0) * row_bytes_k
-                    : (const uint8_t*)g.w + ((int64_t)t.e * g.M + t.c0) * row_bytes_k;
+                    : (const uint8_t*)g.w + ((int64_t)t.e * g.M + c0) * row_bytes_k;
         const int nl = is_r ? LR : 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -222,7 +90,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
         }
     } else {
         // 512-byte rows of 256 columns: two rows a DMA
-        const int cols = is_r ? g.M : C, first = is_r ? t.r0 : t.c0, ld = 2 * cols;
+        const int cols = is_r ? g.M : C, first = is_r ? t.r0 : c0, ld = 2 * cols;
         base = is_r ? (const uint8_t*)g.x + (int64_t)t.p0 * ld
                     : (const uint8_t*)g.w + (kOp == kGroupedDgrad ? (int64_t)t.e * g.M : (int64_t)t.p0) * ld;
         advance = (int64_t)kStep * ld;
@@ -240,9 +108,9 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     uint32_t so = 0;
     int64_t slast = 0;
     if constexpr (kSD > 0) {
-        const int kb = g.K / 32, valid = is_r ? nrows : min(kTile, C - t.c0);
+        const int kb = g.K / 32, valid = is_r ? nrows : min(kTile, C - c0);
         const uint8_t* s0 = is_r ? (const uint8_t*)g.x_scales + (int64_t)(t.p0 + t.r0) * kb
-                                 : (const uint8_t*)g.w_scales + ((int64_t)t.e * g.M + t.c0) * kb;
+                                 : (const uint8_t*)g.w_scales + ((int64_t)t.e * g.M + c0) * kb;
         const uint8_t* end = is_r ? (const uint8_t*)g.x_scales + (int64_t)g.P * kb
                                   : (const uint8_t*)g.w_scales + (int64_t)g.E * g.M * kb;
         const uint32_t d = kSD == 2 ? (uint32_t)((uintptr_t)s0 & 3) : 0u;
@@ -267,18 +135,18 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
         if (kSD != 1 && k == nk - 1 && rem < kStep) {   // (kSD 1: whole steps)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (!is_r || j < LR) dma16(tail_off(j), b, l0 + 1024u * j);
+                if (!is_r || j < LR) lds_dma16(tail_off(j), b, l0 + 1024u * j);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (!is_r || j < LR) dma16(off[j], b, l0 + 1024u * j);
+                if (!is_r || j < LR) lds_dma16(off[j], b, l0 + 1024u * j);
         }
         if constexpr (kSD > 0) {
             const uint32_t ls = l_ring + slot + 2 * kOperand + (is_r ? 0u : 1024u) + 256u * (uint32_t)lw;
-            dma4(so, sbase + 4 * (int64_t)k, ls);
+            lds_dma4(so, sbase + 4 * (int64_t)k, ls);
             if constexpr (kSD == 2) {
                 const int64_t last = slast - 4 * (int64_t)k;   // (the last dword of the array)
-                dma4((uint32_t)min((int64_t)so + 4, last), sbase + 4 * (int64_t)k, ls + 2048u);
+                lds_dma4((uint32_t)min((int64_t)so + 4, last), sbase + 4 * (int64_t)k, ls + 2048u);
             }
         }
     };
@@ -301,7 +169,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
             return (uint32_t)(row * 4) + (q >> 2) * 2048u + (q & 3u);
         };
         asr = l_ring + 2 * kOperand + at(g.x_scales, t.p0 + t.r0, 16 * wm + i);
-        asc = l_ring + 2 * kOperand + 1024 + at(g.w_scales, (int64_t)t.e * g.M + t.c0, 64 * wn + 16 * iq + ib);
+        asc = l_ring + 2 * kOperand + 1024 + at(g.w_scales, (int64_t)t.e * g.M + c0, 64 * wn + 16 * iq + ib);
     }
     // A step's c fragments are read while the one before is multiplied, an r fragment right
     // after the last product of the one that it replaces: a read has most of a step to arrive
@@ -356,14 +224,14 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     auto wait_stage = [&](int after) __attribute__((always_inline)) {
         if (is_r) {
             constexpr int L = LR + kSD;
-            if (after >= S - 3) wait_barrier<(S - 3) * L>();
-            else if (after == 1) wait_barrier<L>();
-            else wait_barrier<0>();
+            if (after >= S - 3) loads_barrier<(S - 3) * L>();
+            else if (after == 1) loads_barrier<L>();
+            else loads_barrier<0>();
         } else {
             constexpr int L = 4 + kSD;
-            if (after >= S - 3) wait_barrier<(S - 3) * L>();
-            else if (after == 1) wait_barrier<L>();
-            else wait_barrier<0>();
+            if (after >= S - 3) loads_barrier<(S - 3) * L>();
+            else if (after == 1) loads_barrier<L>();
+            else loads_barrier<0>();
         }
     };
     if (nk > 0) {
@@ -406,11 +274,11 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
             for (int f = 0; f < 4; ++f) acc[m][f] = mma<kT>(fc[0].v[f], fr[m], acc[m][f], fc[0].s[f], sr[m]);
     }
     const int64_t row0 = kRtr ? (int64_t)t.e * g.M + t.r0 : t.p0 + t.r0;
-    const int c = t.c0 + 64 * wn + 16 * gq;
+    const int c = c0 + 64 * wn + 16 * gq;
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
         const int r = 32 * m + 16 * wm + i;
-        if (r < nrows) store16(g, row0 + r, c, C, acc[m]);
+        if (r < nrows) store_row(g, row0 + r, c, C, acc[m]);
     }
 }
 
@@ -418,7 +286,7 @@ template <int kOp, int kT, int kSD>
 __global__ __launch_bounds__(512, 2) void tile_kernel(GroupedArgs g, int nct) {
     __shared__ __attribute__((aligned(1024))) uint8_t ring[Ring<kT, kSD>::kStages * Ring<kT, kSD>::kStage];
     TileAt t;
-    if (!find_tile<kOp>(g, nct, t)) return;
+    if (!(kOp == kGroupedWgrad ? find_wgrad_tile(g, nct, t) : find_tile<kTile>(g, nct, t))) return;
     const int rows = (kOp == kGroupedWgrad ? g.M : t.n) - t.r0;
     if (rows > 192) run_tile<kOp, kT, kSD, 8>(g, t, ring);
     else if (rows > 128) run_tile<kOp, kT, kSD, 6>(g, t, ring);

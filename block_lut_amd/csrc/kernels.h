@@ -195,7 +195,11 @@ struct GroupedArgs {
     int zero_rest;             // forward, dgrad: rows of no group are set to zero (else not written)
 };
 int launch_grouped(const GroupedArgs& g, hipStream_t s);
-// grouped_tile.hip: every product but MXFP4 matrices with bf16 rows
+// grouped_tile.hip: every product but MXFP4 matrices with bf16 rows; grouped_mx.hip: those;
+// grouped_few.hip: any forward product, and where it is the faster one
+bool grouped_few_rows(const GroupedArgs& g);
 int launch_grouped_tile(const GroupedArgs& g, hipStream_t s);
+int launch_grouped_mx(const GroupedArgs& g, hipStream_t s);
+int launch_grouped_few(const GroupedArgs& g, hipStream_t s);
 
 }  // namespace lutmoe_host
