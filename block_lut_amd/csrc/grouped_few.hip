@@ -118,9 +118,12 @@ int few_launch(const GroupedArgs& g, hipStream_t s) {
 // One wave's K steps of MXFP4 (256 columns): LDS that the wave has to itself, filled by DMA.  Rows
 // of the matrix as 8 16-byte pieces on consecutive lanes (a load of 16 bytes from 16 rows on
 // consecutive lanes takes the address unit a line a lane, which bounds it: 3.3 TB/s at 14 loads
-// per 4 KB), piece p of row r at p ^ (r / 2 % 8); 16 bytes of scales a row from the dword that holds
-// the step's first one; bf16 rows as 32 chunks, chunk c of row r at c ^ r % 16, MXFP4 ones as the
+// per 4 KB), piece p of row r at p ^ swz(r); 16 bytes of scales a row from the dword that holds
+// the step's first one; bf16 rows as 32 chunks, chunk c of row r at c ^ xswz(r), MXFP4 ones as the
 // matrix.
+__device__ __forceinline__ int swz(int r) { return 2 * quad_order(r & 15) | ((r >> 1) & 1); }
+__device__ __forceinline__ int xswz(int r) { return ((r >> 1) & 4) | (r & 3); }
+
 template <bool kX4, int CR, int kRows>
 struct MxStage {
     static constexpr int kXLoads = kX4 ? (kRows + 7) / 8 : (kRows + 1) / 2;
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(64 * W) void few_mx_kernel(GroupedArgs g, int nct) 
     auto column = [&](int f, int r) __attribute__((always_inline)) {
         return min(4 * CR * (r >> 2) + 4 * f + (r & 3), g.M - 1 - c0);
     };
-    auto pieces = [&](int r) __attribute__((always_inline)) { return (lane & 7) ^ ((r >> 1) & 7); };
+    auto pieces = [&](int r) __attribute__((always_inline)) { return (lane & 7) ^ swz(r); };
     uint32_t wo[CR][2], xo[St::kXLoads];
 #pragma unroll
     for (int f = 0; f < CR; ++f)
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(64 * W) void few_mx_kernel(GroupedArgs g, int nct) 
     for (int d = 0; d < St::kXLoads; ++d) {
         const int r = kX4 ? 8 * d + (lane >> 3) : 2 * d + (lane >> 5);
         const uint32_t row = (uint32_t)min(r, nrows - 1);
-        xo[d] = kX4 ? row * row_b + 16u * (uint32_t)pieces(r) : row * 4 * row_b + 16u * (uint32_t)((lane & 31) ^ (r & 15));
+        xo[d] = kX4 ? row * row_b + 16u * (uint32_t)pieces(r) : row * 4 * row_b + 16u * (uint32_t)((lane & 31) ^ xswz(r));
     }
     // scales: lane l dword l % 4 of row l / 4's window, which starts at the dword that holds the step's
     // first byte; `so` from the aligned base, never past the array's last dword
@@ -209,16 +212,16 @@ __global__ __launch_bounds__(64 * W) void few_mx_kernel(GroupedArgs g, int nct) 
 #pragma unroll
         for (int d = 0; d < St::kXLoads; ++d) {
             if constexpr (kX4) lds_dma16(in_row(xo[d], pieces(8 * d + (lane >> 3)), 1), xbase + 128 * (int64_t)s, l0 + St::kX + 1024 * d);
-            else lds_dma16(in_row(xo[d], (lane & 31) ^ ((2 * d + (lane >> 5)) & 15), 4), xbase + 512 * (int64_t)s, l0 + St::kX + 1024 * d);
+            else lds_dma16(in_row(xo[d], (lane & 31) ^ xswz(2 * d + (lane >> 5)), 4), xbase + 512 * (int64_t)s, l0 + St::kX + 1024 * d);
         }
         if constexpr (kX4) scale_dma(xs, xso, s, l0 + St::kXs);
     };
 
     // ---- reads: lane (i, q) blocks 2 q, 2 q + 1 of row i (rows past the item's: its last loaded one)
     const int xi = min(i, St::kXLoads * (kX4 ? 8 : 2) - 1);
-    const uint32_t wr = ring + (uint32_t)(i * 128 + 16 * ((2 * q) ^ ((i >> 1) & 7)));
-    const uint32_t xr = ring + St::kX + (kX4 ? (uint32_t)(xi * 128 + 16 * ((2 * q) ^ ((xi >> 1) & 7)))
-                                             : (uint32_t)(xi * 512 + 16 * ((8 * q) ^ (xi & 15))));
+    const uint32_t wr = ring + (uint32_t)(i * 128 + 16 * ((2 * q) ^ swz(i)));
+    const uint32_t xr = ring + St::kX + (kX4 ? (uint32_t)(xi * 128 + 16 * ((2 * q) ^ swz(xi)))
+                                             : (uint32_t)(xi * 512 + 16 * ((8 * q) ^ xswz(xi))));
     uint32_t wsr[CR];
 #pragma unroll
     for (int f = 0; f < CR; ++f)

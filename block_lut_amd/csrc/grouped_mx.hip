@@ -4,9 +4,9 @@
 //
 // A CTA is 8 waves on 256 columns and up to 128 rows of one group, a wave 32 columns of all
 // rows.  K steps of 128 columns through a ring of stages filled by LDS DMA: each wave's codes
-// and scales (32 matrix rows of 64 bytes, 16-byte piece p of row r at p ^ (r / 4 % 4); two
+// and scales (32 matrix rows of 64 bytes, 16-byte piece p of row r at p ^ (-(r / 4) % 4); two
 // dwords of scales a row, so that they may start anywhere), and the rows that all waves share
-// (256 bytes each, chunk c of row r at c ^ r % 16): reads without bank conflicts.  Lane (i, q)
+// (256 bytes each, chunk c of row r at c ^ swz(r)): reads without bank conflicts.  Lane (i, q)
 // holds block 4 s + q of its two matrix rows, and the rows' fragment j of the step is their
 // columns 32 q + 8 j .. + 7 (the same permutation of k on both sides).  A fragment is read
 // right after the last product of the one that it replaces.
@@ -28,6 +28,8 @@ struct Ring {
     static constexpr int kStages = 3;
     static constexpr int kLoads = 3 + kLoadF / 2;         // DMAs a wave and stage
 };
+
+__device__ __forceinline__ int swz(int r) { return 4 * quad_order(r & 15) | (r & 3); }
 
 template <int RF>
 __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, uint8_t* ring) {
@@ -52,7 +54,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
             return (uint32_t)min(8 * ((r >> 2) & 3) + 4 * (r >> 4) + (r & 3), g.M - 1 - c_first);
         };
         const uint8_t* wbase = (const uint8_t*)g.w + wrow0 * row_b;
-        const int wpiece = (lane & 3) ^ (lane >> 4);
+        const int wpiece = (lane & 3) ^ quad_order(lane >> 2);
         uint32_t wo[2];
 #pragma unroll
         for (int d = 0; d < 2; ++d) wo[d] = column(16 * d + (lane >> 2)) * row_b + 16u * (uint32_t)wpiece;
@@ -69,7 +71,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
 #pragma unroll
         for (int j = 0; j < LX; ++j) {
             const int r = 4 * (LX * wv + j) + q;
-            xo[j] = (uint32_t)min(r, nrows - 1) * (uint32_t)(2 * g.K) + 16u * (uint32_t)(i ^ (r & 15));
+            xo[j] = (uint32_t)min(r, nrows - 1) * (uint32_t)(2 * g.K) + 16u * (uint32_t)(i ^ swz(r));
         }
         auto issue = [&](int k, uint32_t slot) __attribute__((always_inline)) {
             const bool tail = k == nk - 1;   // pieces past the row's end: the step's first piece again
@@ -81,13 +83,13 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
             const uint32_t lx = l_ring + slot + Rg::kX + (uint32_t)(LX * wv) * 1024u;
 #pragma unroll
             for (int j = 0; j < LX; ++j) {
-                const int c = i ^ ((4 * (LX * wv + j) + q) & 15);
+                const int c = i ^ swz(4 * (LX * wv + j) + q);
                 lds_dma16(xo[j] - (tail && c >= 4 * rem ? 16u * (uint32_t)c : 0u), xbase + 256 * (int64_t)k, lx + 1024u * j);
             }
         };
         // ---- reads
-        const uint32_t ar = l_ring + Rg::kX + (uint32_t)(i * 256 + 16 * ((4 * q) ^ i));
-        const uint32_t aw = l_ring + (uint32_t)(wv * Rg::kWave + i * 64 + 16 * (q ^ (i >> 2)));
+        const uint32_t ar = l_ring + Rg::kX + (uint32_t)(i * 256 + 16 * ((4 * q) ^ swz(i)));
+        const uint32_t aw = l_ring + (uint32_t)(wv * Rg::kWave + i * 64 + 16 * (q ^ quad_order(i)));
         uint32_t as[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f)

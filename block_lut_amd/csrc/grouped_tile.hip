@@ -8,12 +8,14 @@
 // A CTA is 8 waves (2 along r x 4 along c, a wave 128 x 64) on a tile of up to 256 x 256.
 // K goes in steps of 64 bytes a row (32 columns, MXFP4: 128) through a ring of stages of 32 KB,
 // filled by 16-byte LDS DMA; a step's fragments are read while the one before is multiplied.
-// Layouts of a stage (all reads without bank conflicts):
-//   k-contiguous  64-byte rows, 16-byte chunk q of row r at q ^ (r / 4 % 4) (c: q ^ (r / 16 % 4))
-//   transposed    512-byte rows of 256 columns, read by the transposing LDS read
-//                 (ds_read_b64_tr_b16: 4 rows x 16 columns -> 4 elements of a column a lane)
-// Fragment f of the c operand takes the columns 16 (i / 4) + 4 f + i % 4 (i its row), so that a
-// lane's accumulators are 16 consecutive results of one row: whole 16-byte stores.
+// Layouts of a stage (reads without bank conflicts):
+//   k-contiguous  64-byte rows, 16-byte chunk q of row r at q ^ (-(r / 4) % 4)
+//   transposed    512-byte rows of 256 columns (chunk q of row r at q ^ (2 (r % 4) + 8 (r / 8 % 2))), read
+//                 by the transposing LDS read (ds_read_b64_tr_b16: 4 rows x 16 columns -> 4
+//                 elements of a column a lane)
+// A lane's accumulators become 16 consecutive results of one row, whole 16-byte stores: a
+// k-contiguous c operand's rows are put in that order on their way to LDS, a transposed one's
+// results exchanged between the lane groups at the end.
 // Ragged groups: a group's last tile computes 64, 128 or 192 rows where that is enough (the
 // two waves of a column block take alternate 16-row fragments).
 #include "grouped.h"
@@ -84,8 +86,9 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
         const int nl = is_r ? LR : 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int row = min(16 * (nl * lw + j) + (lane >> 2), valid - 1);
-            const int chunk = (lane & 3) ^ (is_r ? lane >> 4 : j);
+            // (a c fragment's row i is column 16 (i / 4) + 4 j + i % 4 of the wave's 64)
+            const int row = min(is_r ? 16 * (nl * lw + j) + (lane >> 2) : 64 * lw + 16 * (lane >> 4) + 4 * j + ((lane >> 2) & 3), valid - 1);
+            const int chunk = (lane & 3) ^ quad_order(lane >> 2);
             off[j] = (uint32_t)row * (uint32_t)row_bytes_k + 16u * (uint32_t)chunk;
         }
     } else {
@@ -97,8 +100,7 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = 2 * (4 * lw + j) + (lane >> 5);
-            const int h = is_r ? ((row & 3) << 1) | (row & 8) : (row & 1) | ((row & 2) << 2);
-            const int chunk = min(first / 8 + ((lane & 31) ^ h), cols / 8 - 1);
+            const int chunk = min(first / 8 + ((lane & 31) ^ (((row & 3) << 1) | (row & 8))), cols / 8 - 1);
             off[j] = (uint32_t)row * (uint32_t)ld + 16u * (uint32_t)chunk;
         }
     }
@@ -123,25 +125,18 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     // step's first chunk (row) instead
     auto tail_off = [&](int j) __attribute__((always_inline)) {
         if ((is_r && !kRtr) || (!is_r && !kCtr)) {
-            const int chunk = (lane & 3) ^ (is_r ? lane >> 4 : j);
+            const int chunk = (lane & 3) ^ quad_order(lane >> 2);
             return off[j] - (chunk * kChunk >= rem ? 16u * (uint32_t)chunk : 0u);
         }
         const int row = 2 * (4 * lw + j) + (lane >> 5);
         return off[j] - (row >= rem ? (uint32_t)row * (uint32_t)(2 * (is_r ? g.M : C)) : 0u);
     };
-    auto issue = [&](int k, uint32_t slot) __attribute__((always_inline)) {
+    // part j of stage k's loads
+    auto issue_part = [&](int k, uint32_t slot, int j) __attribute__((always_inline)) {
         const uint8_t* b = base + (int64_t)k * advance;
         const uint32_t l0 = l_ring + slot + (is_r ? (uint32_t)(LR * lw) * 1024u : (uint32_t)kOperand + (uint32_t)lw * 4096u);
-        if (kSD != 1 && k == nk - 1 && rem < kStep) {   // (kSD 1: whole steps)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!is_r || j < LR) lds_dma16(tail_off(j), b, l0 + 1024u * j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!is_r || j < LR) lds_dma16(off[j], b, l0 + 1024u * j);
-        }
-        if constexpr (kSD > 0) {
+        if (!is_r || j < LR) lds_dma16(kSD != 1 && k == nk - 1 && rem < kStep ? tail_off(j) : off[j], b, l0 + 1024u * j);   // (kSD 1: whole steps)
+        if (kSD > 0 && j == 0) {
             const uint32_t ls = l_ring + slot + 2 * kOperand + (is_r ? 0u : 1024u) + 256u * (uint32_t)lw;
             lds_dma4(so, sbase + 4 * (int64_t)k, ls);
             if constexpr (kSD == 2) {
@@ -155,10 +150,12 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     const int i = lane & 15, gq = lane >> 4, wm = wv >> 2, wn = wv & 3;
     const int iq = i >> 2, ib = i & 3;
     uint32_t ar, ac;
-    if constexpr (kRtr) ar = (uint32_t)((8 * gq + iq) * 512 + 16 * ((2 * wm + (ib >> 1)) ^ ((iq << 1) | ((gq & 1) << 3))) + 8 * (ib & 1));
-    else ar = (uint32_t)((16 * wm + i) * 64 + 16 * (gq ^ iq));
-    if constexpr (kCtr) ac = (uint32_t)((8 * gq + iq) * 512 + 16 * ((8 * wn + 2 * ib) ^ ((iq & 1) | ((iq >> 1) << 3))));
-    else ac = (uint32_t)((64 * wn + 16 * iq + ib) * 64 + 16 * (gq ^ iq));
+    // (transposed: rows 8 gq + 4 s + iq, 8 bytes of them at column 4 ib of a fragment's 16)
+    const uint32_t at_tr = (uint32_t)((8 * gq + iq) * 512 + 8 * (ib & 1)), h_tr = (uint32_t)((iq << 1) | ((gq & 1) << 3));
+    if constexpr (kRtr) ar = at_tr + 16u * ((uint32_t)(2 * wm + (ib >> 1)) ^ h_tr);
+    else ar = (uint32_t)((16 * wm + i) * 64 + 16 * (gq ^ quad_order(i)));
+    if constexpr (kCtr) ac = at_tr + 16u * ((uint32_t)(8 * wn + (ib >> 1)) ^ h_tr);
+    else ac = (uint32_t)((64 * wn + i) * 64 + 16 * (gq ^ quad_order(i)));
     ar += l_ring;
     ac += l_ring + kOperand;
     uint32_t asr = 0, asc = 0;   // MXFP4: scale byte addresses
@@ -181,8 +178,8 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
     u32x4_t fr[MF];
     int sr[MF];
     auto read_c = [&](uint32_t slot, ColFrags& F, int f) __attribute__((always_inline)) {
-        if constexpr (kCtr) F.v[f] = lds_tr(((ac + slot) ^ (uint32_t)(16 * (f >> 1))) + 8 * (f & 1));
-        else F.v[f] = lds_quad(ac + slot + 256 * f);
+        if constexpr (kCtr) F.v[f] = lds_tr((ac + slot) ^ (uint32_t)(32 * f));
+        else F.v[f] = lds_quad(ac + slot + 1024 * f);
         F.s[f] = 0;
         if constexpr (kSD > 0) F.s[f] = *(lds_byte_t)(asc + slot + 16 * f);
     };
@@ -235,7 +232,9 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
         }
     };
     if (nk > 0) {
-        for (int k = 0; k < min(S - 1, nk); ++k) issue(k, (uint32_t)k * Rg::kStage);
+        for (int k = 0; k < min(S - 1, nk); ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) issue_part(k, (uint32_t)k * Rg::kStage, j);
         wait_stage(min(S - 2, nk - 1));   // stage 0 has landed (the count of S - 3 stages waits for one more)
 #pragma unroll
         for (int f = 0; f < 4; ++f) read_c(0, fc[0], f);
@@ -249,14 +248,21 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
         };
         auto step = [&](ColFrags& F0, ColFrags& F1, int k) __attribute__((always_inline)) {
             wait_stage(min(S - 3, nk - 2 - k));
-            if (k - 1 + S < nk) issue(k - 1 + S, prev);
+            const bool refill = k - 1 + S < nk;
+            // (what is loaded and read goes behind products, which hide its issue)
 #pragma unroll
             for (int m = 0; m < MF; ++m) {
-                if (m < 4 && MF >= 4) read_c(next, F1, m);
-                else if (m < 2) { read_c(next, F1, 2 * m); read_c(next, F1, 2 * m + 1); }
 #pragma unroll
                 for (int f = 0; f < 4; ++f) acc[m][f] = mma<kT>(F0.v[f], fr[m], acc[m][f], F0.s[f], sr[m]);
                 read_r(next, m);
+                constexpr int kPer = MF < 4 ? 2 : 1;   // parts of the rest behind a fragment's products
+                if (kPer * m < 4) {
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        read_c(next, F1, kPer * m + j);
+                        if (refill) issue_part(k - 1 + S, prev, kPer * m + j);
+                    }
+                }
                 __builtin_amdgcn_sched_barrier(0);   // (a read hoisted higher takes registers that are not there)
             }
             prev = after_slot(prev);
@@ -278,6 +284,17 @@ __device__ __forceinline__ void run_tile(const GroupedArgs& g, const TileAt& t, 
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
         const int r = 32 * m + 16 * wm + i;
+        // (transposed c fragments are 16 columns each: a lane's results made consecutive)
+        if constexpr (kCtr)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                float v0 = acc[m][0][d], v1 = acc[m][1][d], v2 = acc[m][2][d], v3 = acc[m][3][d];
+                transpose4(v0, v1, v2, v3);
+                acc[m][0][d] = v0;
+                acc[m][1][d] = v1;
+                acc[m][2][d] = v2;
+                acc[m][3][d] = v3;
+            }
         if (r < nrows) store_row(g, row0 + r, c, C, acc[m]);
     }
 }
