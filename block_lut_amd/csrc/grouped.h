@@ -44,46 +44,55 @@ __device__ __forceinline__ int wave_scan(int v) {
 // tiles go along with a column tile.  Every wave finds it by itself: the tiles of 64 groups
 // at a time summed up across its lanes (up to 64 groups: one load of the offsets, one sum).
 template <int kHeight>
-__device__ __forceinline__ bool find_tile(const GroupedArgs& g, int nct, TileAt& t) {
-    const int lane = threadIdx.x & 63, b = blockIdx.x;
-    const int groups = g.E + (g.zero_rest ? 1 : 0);
-    int p0, n, mine, upto, total = 0;
-    auto sums = [&](int e0) __attribute__((always_inline)) {
+struct Tiles {
+    int nct, groups, total, p0, n, mine, upto;
+
+    __device__ __forceinline__ int sums(const GroupedArgs& g, int e0) {
+        const int lane = threadIdx.x & 63;
         group_rows(g, e0 + lane, p0, n);
         if (e0 + lane >= groups) n = 0;
         mine = (n + kHeight - 1) / kHeight;
         upto = wave_scan(mine);
         return __builtin_amdgcn_readlane(upto, 63);
-    };
-    for (int e0 = 0; e0 < groups; e0 += 64) total += sums(e0);
-    total *= nct;
-    const int per = (total + 7) / 8, i = (b & 7) * per + (b >> 3);
-    if ((b >> 3) >= per || i >= total) return false;
-    int before = 0;
-    for (int e0 = 0; e0 < groups; e0 += 64) {
-        if (groups > 64) sums(e0);
-        const uint64_t m = __ballot(i < before + upto * nct);
-        if (m) {
-            const int l = __builtin_ctzll(m);
-            t.e = e0 + l;
-            t.p0 = __builtin_amdgcn_readlane(p0, l);
-            t.n = __builtin_amdgcn_readlane(n, l);
-            const int mt = __builtin_amdgcn_readlane(mine, l);
-            const int in = i - before - (__builtin_amdgcn_readlane(upto, l) - mt) * nct;
-            if (mt == 1) {
-                t.ct = in;
-                t.r0 = 0;
-            } else {
-                const int grp = in / (8 * nct), size = min(8, mt - 8 * grp), rem = in - grp * 8 * nct;
-                t.ct = rem / size;
-                t.r0 = (8 * grp + rem - t.ct * size) * kHeight;
-            }
-            // (decreasing offsets can count more tiles than an int holds)
-            return (uint32_t)t.r0 < (uint32_t)t.n && (uint32_t)t.ct < (uint32_t)nct;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63) * nct;
     }
-    return false;
+    __device__ __forceinline__ Tiles(const GroupedArgs& g, int nct_) : nct(nct_), groups(g.E + (g.zero_rest ? 1 : 0)), total(0) {
+        for (int e0 = 0; e0 < groups; e0 += 64) total += sums(g, e0);
+        total *= nct;
+    }
+    // the tile of CTA b
+    __device__ __forceinline__ bool at(const GroupedArgs& g, int b, TileAt& t) {
+        const int per = (total + 7) / 8, i = (b & 7) * per + (b >> 3);
+        if ((b >> 3) >= per || i >= total) return false;
+        int before = 0;
+        for (int e0 = 0; e0 < groups; e0 += 64) {
+            if (groups > 64) sums(g, e0);
+            const uint64_t m = __ballot(i < before + upto * nct);
+            if (m) {
+                const int l = __builtin_ctzll(m);
+                t.e = e0 + l;
+                t.p0 = __builtin_amdgcn_readlane(p0, l);
+                t.n = __builtin_amdgcn_readlane(n, l);
+                const int mt = __builtin_amdgcn_readlane(mine, l);
+                const int in = i - before - (__builtin_amdgcn_readlane(upto, l) - mt) * nct;
+                if (mt == 1) {
+                    t.ct = in;
+                    t.r0 = 0;
+                } else {
+                    const int grp = in / (8 * nct), size = min(8, mt - 8 * grp), rem = in - grp * 8 * nct;
+                    t.ct = rem / size;
+                    t.r0 = (8 * grp + rem - t.ct * size) * kHeight;
+                }
+                // (decreasing offsets can count more tiles than an int holds)
+                return (uint32_t)t.r0 < (uint32_t)t.n && (uint32_t)t.ct < (uint32_t)nct;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63) * nct;
+        }
+        return false;
+    }
+};
+template <int kHeight>
+__device__ __forceinline__ bool find_tile(const GroupedArgs& g, int nct, TileAt& t) {
+    return Tiles<kHeight>(g, nct).at(g, blockIdx.x, t);
 }
 
 // 4 Q results of one row from its column c on (C columns in all): whole vectors where the
@@ -151,13 +160,29 @@ __device__ __forceinline__ u32x4_t widen(uint32_t codes, uint32_t byte) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 3))};
 }
 
-// LDS DMA: 16 (4) bytes a lane from sbase + voff to m0 + 16 (4) x lane.  The base is an SGPR
-// pair, which carries the 5 wait states that a VALU write of it needs.
+// LDS DMA: 16 (4) bytes a lane from sbase + voff to m0 + 16 (4) x lane.  The loads are written in
+// asm, so they carry the 5 wait states themselves that a vector instruction's write of their scalar operands
+// needs (the compiler reloads those from vector registers where it runs short).
 __device__ __forceinline__ void lds_dma16(uint32_t voff, const void* sbase, uint32_t m0) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 __device__ __forceinline__ void lds_dma4(uint32_t voff, const void* sbase, uint32_t m0) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+}
+// The same from a buffer, at voff + soff; at and beyond its end (descriptor: the bytes from `base`
+// on): zeros.
+__device__ __forceinline__ u32x4_t lds_source(const uint8_t* base, uint32_t bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)base;
+    u32x4_t d = {(uint32_t)__builtin_amdgcn_readfirstlane((int)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufWord3};
+    asm volatile("" : "+s"(d));   // (not in vector registers)
+    return d;
+}
+__device__ __forceinline__ void lds_dma16(uint32_t voff, const u32x4_t& src, uint32_t soff, uint32_t m0) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(voff), "s"(src), "s"(soff), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void lds_dma4(uint32_t voff, const u32x4_t& src, uint32_t soff, uint32_t m0) {
+    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" : : "v"(voff), "s"(src), "s"(soff), "{m0}"(m0) : "memory");
 }
 // At most kAfter of the wave's loads still in flight, then barrier.  Every wave has waited for
 // the LDS reads of what it multiplied before.
@@ -173,26 +198,13 @@ __device__ __forceinline__ void loads_barrier() {
 // is made of this.
 __device__ __forceinline__ int quad_order(int i) { return (-(i >> 2)) & 3; }
 
-// Exchange 4 x 4 values between the lane groups q and the registers f: lane group q has
-// v[q'] of group f afterwards where it had v[f] of group q'.
-__device__ __forceinline__ void transpose4(float& v0, float& v1, float& v2, float& v3) {
-    uint32_t a[4] = {__float_as_uint(v0), __float_as_uint(v1), __float_as_uint(v2), __float_as_uint(v3)};
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-        const auto r = __builtin_amdgcn_permlane32_swap(a[f], a[f + 2], false, false);
-        a[f] = r[0];
-        a[f + 2] = r[1];
-    }
-#pragma unroll
-    for (int f = 0; f < 4; f += 2) {
-        const auto r = __builtin_amdgcn_permlane16_swap(a[f], a[f + 1], false, false);
-        a[f] = r[0];
-        a[f + 1] = r[1];
-    }
-    v0 = __uint_as_float(a[0]);
-    v1 = __uint_as_float(a[1]);
-    v2 = __uint_as_float(a[2]);
-    v3 = __uint_as_float(a[3]);
+// Four bytes of each of four rows' words -> one byte of each: lane group f holds the word of row f,
+// group q gets byte q of the words 0 .. 3 (`pick`: 0x0c0c0000 | (4 + q) << 8 | q).
+__device__ __forceinline__ uint32_t bytes4(uint32_t v, uint32_t pick) {
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);          // words 0 1 0 1, 2 3 2 3
+    const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);    // 0 everywhere, 1
+    const auto b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);    // 2, 3
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[1], b[0], pick), __builtin_amdgcn_perm(a[1], a[0], pick), 0x05040100u);
 }
 
 typedef __attribute__((address_space(3))) const u32x4_t* lds_quad_t;

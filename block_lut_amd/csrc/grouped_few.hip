@@ -357,13 +357,14 @@ namespace lutmoe_host {
 
 // Up to how many rows a group the kernels here are taken (the tiles read a matrix once for up to
 // 32, 128 or 256 rows): while its groups are short, or their tiles would leave most CUs
-// without one.  us, these / the tiles: 60 matrices 2816 x 2048 with 512 (1024) rows, MXFP4 and bf16 rows
-// 50.6 / 49.9 (71 / 52), MXFP4 rows 37.9 / 45.9 (46.7 / 47.3); 1 matrix 2816 x 2048 with 256 rows 13.2 / 15.4 and
-// 7.9 / 21.5; 20000 x 1024 with 64 rows 14.3 / 10.0 and 9.8 / 8.6.
+// without one.  us, these / the tiles: 60 matrices 2816 x 2048, bf16 with 240 (960) rows 125 / 146 (191 / 145),
+// MXFP4 rows 1200 (1920) 50 / 56 (60 / 57), MXFP4 and bf16 rows 512 (1024) 50.6 / 49.9 (71 / 52); one matrix
+// 4096 x 4096, bf16 64 (128) rows 25 / 32 (46 / 36), MXFP4 rows 256 16 / 21; 8 matrices 2816 x 2048, bf16 128
+// rows 35 / 27, MXFP4 rows 512 16 / 13.
 bool grouped_few_rows(const GroupedArgs& g) {
     const Items it = items_of(g);
-    const int rows = !g.w_scales ? 16 : g.x_scales ? 12 : 8;
-    return it.rows <= rows || it.count <= (g.w_scales ? 4096 : 2816);
+    const int rows = !g.w_scales ? 10 : g.x_scales ? 28 : 8;
+    return it.rows <= rows || it.count <= (g.w_scales ? 4096 : 1280);
 }
 
 int launch_grouped_few(const GroupedArgs& g, hipStream_t s) {
