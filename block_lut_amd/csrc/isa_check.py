@@ -1,17 +1,20 @@
 """Hazard check over the gfx950 code of liblutmoe's own objects.
 
-The kernels issue their LDS-DMA loads (global_load_lds_*) as inline asm, so the
-compiler's hazard recognizer does not look at them.  On gfx950 (a GFX9 target) a
+The kernels issue their LDS-DMA loads (global_load_lds_*, buffer_load_* ... lds) as
+inline asm, so the compiler's hazard recognizer does not look at them.  On gfx950 (a GFX9 target) a
 VMEM instruction that reads an SGPR written by a VALU instruction (v_readlane,
 v_readfirstlane, a VOP3 carry-out, a compare) needs 5 wait states in between:
 the compiler puts `s_nop 4` in front of its own loads in that case.  Without
-them the load may use the SGPR's old value as its base address.
+them the load may use the SGPR's old value as its base address.  The same holds for
+the tiles' matrix products: one that reads a vector register written by another
+vector instruction needs 2 wait states.
 
 This module disassembles the device code object embedded in each built object
 (llvm-objcopy, clang-offload-bundler, llvm-objdump from the ROCm toolchain) and
 walks back from every LDS-DMA load along every path into it (fall-through and
 branches), for 5 wait states, looking for a VALU write of an SGPR the load reads
-(its base pair and M0).
+(its base pair or descriptor, its offset and M0), and alike from every matrix product for
+2, looking for a VALU write of a register it reads.
 
     python -m block_lut_amd.csrc.isa_check      # checks block_lut_amd/_build/*.o
 """
@@ -29,12 +32,14 @@ PKG = os.path.dirname(HERE)
 LLVM = "/opt/rocm/llvm/bin"
 TARGET = "hipv4-amdgcn-amd-amdhsa--gfx950"
 WAIT_STATES = 5
+PRODUCT_WAIT_STATES = 2
 
 _INSN = re.compile(r"^\s+([a-z_0-9]+)(.*?)\s*//\s*([0-9A-Fa-f]+):")
 _FUNC = re.compile(r"^([0-9a-f]+) <(.+)>:")
 _TARGET = re.compile(r"<(.+)\+0x([0-9a-f]+)>\s*$")
 _SPAIR = re.compile(r"^s\[(\d+):(\d+)\]$")
 _SREG = re.compile(r"^s(\d+)$")
+_VREG = re.compile(r"^([va])(?:\[(\d+):(\d+)\]|(\d+))$")
 
 
 def _sregs(tok: str) -> set:
@@ -45,6 +50,14 @@ def _sregs(tok: str) -> set:
     if _SREG.match(tok) or tok in ("m0", "vcc"):
         return {tok}
     return set()
+
+
+def _vregs(tok: str) -> set:
+    m = _VREG.match(tok.split()[0]) if tok.strip() else None
+    if not m:
+        return set()
+    a = int(m.group(2) or m.group(4))
+    return {f"{m.group(1)}{i}" for i in range(a, int(m.group(3) or a) + 1)}
 
 
 def _operands(rest: str) -> list:
@@ -62,6 +75,16 @@ def _valu_sgpr_defs(mnem: str, ops: list) -> set:
         defs |= _sregs(ops[1])
     if mnem.startswith("v_cmp") and not mnem.endswith("_e64"):
         defs.add("vcc")
+    return defs
+
+
+def _valu_defs(mnem: str, ops: list) -> set:
+    """What a vector instruction other than a matrix product writes."""
+    defs = _valu_sgpr_defs(mnem, ops)
+    if mnem.startswith("v_") and not mnem.startswith("v_mfma") and ops:
+        defs = defs | _vregs(ops[0])
+        if "swap" in mnem and len(ops) > 1:
+            defs = defs | _vregs(ops[1])
     return defs
 
 
@@ -86,9 +109,10 @@ def disassemble(obj: str) -> str:
 
 
 def find_hazards(text: str) -> list:
-    """(function, address, offending VALU, load) for every LDS-DMA load with a
+    """(function, address, offending VALU, load or product) for every LDS-DMA load with a
     VALU write of one of its SGPRs fewer than WAIT_STATES wait states earlier on
-    some path."""
+    some path, and every matrix product with one of a register it reads fewer than
+    PRODUCT_WAIT_STATES earlier."""
     funcs = {}
     insns = []            # (func, addr, mnemonic, operands)
     cur = None
@@ -119,20 +143,25 @@ def find_hazards(text: str) -> list:
 
     hits = []
     for i, (f, a, mn, ops, _) in enumerate(insns):
-        if not mn.startswith("global_load_lds"):
+        if mn.startswith("global_load_lds") or (mn.startswith("buffer_load") and ops and ops[-1].endswith(" lds")):
+            used, need = {"m0"}, WAIT_STATES
+            for o in ops[1:]:
+                used |= _sregs(o.split()[0])
+        elif mn.startswith("v_mfma"):
+            used, need = set(), PRODUCT_WAIT_STATES
+            for o in ops[1:]:
+                used |= _vregs(o)
+        else:
             continue
-        used = {"m0"}
-        for o in ops[1:]:
-            used |= _sregs(o)
         stack = [(p, 0) for p in preds(i)]
         seen = set()
         while stack:
             j, ws = stack.pop()
-            if ws >= WAIT_STATES or (j, ws) in seen:
+            if ws >= need or (j, ws) in seen:
                 continue
             seen.add((j, ws))
             _, aj, mj, oj, _ = insns[j]
-            if _valu_sgpr_defs(mj, oj) & used:
+            if _valu_defs(mj, oj) & used:
                 hits.append((f, a, f"{mj} {', '.join(oj)}", f"{mn} {', '.join(ops)}"))
                 break
             step = int(oj[0], 0) + 1 if mj == "s_nop" and oj else 1
