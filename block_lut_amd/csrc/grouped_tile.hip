@@ -22,12 +22,13 @@
 //                 by the transposing LDS read (ds_read_b64_tr_b16: 4 rows x 16 columns -> 4
 //                 elements of a column a lane)
 // CTAs stay for further tiles: the next tile's first loads go out in front of a tile's stores (64
-// matrices' gradients, 2816 x 2048 from 192 rows each: 308 us, a CTA a tile 318; stored without LDS 401).
+// matrices' gradients, 2816 x 2048 from 192 rows each: 308 us, a CTA a tile 318; results stored straight from
+// the accumulators 407).
 // Ragged groups: a group's last tile computes 64, 128 or 192 rows where that is enough (the
 // two waves of a column block take alternate 16-row fragments).
 // Measured: bf16 8192 rows of 8 matrices 28672 x 4096 1670 us (1150 TFLOP/s; the clock falls to 1.6 GHz
 // under it), 12288 rows of 64 matrices 2816 x 2048 190 us (4.5 TB/s), MXFP4 rows 700 us and 78 us; the gradients of
-// those rows 1970 and 185 us (dgrad), 1900 and 308 us (wgrad, 738 MB written).
+// those rows 1970 and 185 us (dgrad), 1890 and 248 us (wgrad, 738 MB written).
 #include "grouped.h"
 #include <utility>
 
@@ -503,7 +504,13 @@ __device__ __forceinline__ int run_tile(const GroupedArgs& g, const TileAt& t, c
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
                 const int r = 32 * m + 64 / kAt * u;
-                if (16 * wm + lr + r < nrows && c < C) *(u32x4_t*)(base + 2 * (int64_t)r * C + at) = pack(v[u]);
+                u32x4_t* to = (u32x4_t*)(base + 2 * (int64_t)r * C + at);
+                // (wgrad past the caches, whose results are many times their size: 310 -> 248 us for 738 MB; the others'
+                // gain 1 to 3%, and are read next)
+                if (16 * wm + lr + r < nrows && c < C) {
+                    if constexpr (kRtr) __builtin_nontemporal_store(pack(v[u]), to);
+                    else *to = pack(v[u]);
+                }
             }
         }
     };
