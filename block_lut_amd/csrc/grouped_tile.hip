@@ -360,7 +360,7 @@ __device__ __forceinline__ int run_tile(const GroupedArgs& g, const TileAt& t, c
         if constexpr (kSD > 0) {
             const uint32_t(&v)[2] = w < kCH ? sw.c[w] : sw.r[w - kCH];
             const uint32_t u = bytes4(kSD == 3 ? __builtin_amdgcn_alignbyte(v[kSD - 2], v[0], w < kCH ? shift_c : shift_r) : v[0], pick);
-            (w < kCH ? bc[s][w] : br[s][w - kCH]) = kSD == 3 && 32 * gq >= left ? 0u : u;
+            (w < kCH ? bc[s][w] : br[s][w - kCH]) = 32 * gq >= left ? 0u : u;
         }
     };
     f32x4_t acc[MF][N];

@@ -115,6 +115,30 @@ def test_neighbours_are_nan(gpu, M, K, counts):
         _equal(ops.grouped_gemm_wgrad(dyd, xd, off, out_dtype=torch.float32)[e], dy[a:b].T @ x[a:b], "f32")
 
 
+@pytest.mark.parametrize("K", [128, 160, 384, 512])
+@pytest.mark.parametrize("M,counts", [(1850, [0, 1, 64, 65, 130, 300]), (1801, HEIGHTS)])
+def test_mxfp4_rows_next_to_nan(gpu, M, counts, K):
+    """Every second row and every second matrix row is NaN (scale bytes of 255), first of all behind the
+    ends of the others: reductions that end in either half of a stage."""
+    import torch
+    from block_lut_amd import ops
+    E, P = len(counts), sum(counts)
+    rng = np.random.default_rng(M + K)
+    off, o = _off(counts, gpu), G.offsets_of(counts)
+    (wc, ws), (xc, xs) = _mx_ints(rng, (E, M, K)), _mx_ints(rng, (P, K))
+    ref = G.forward(G.mx_decode(xc, xs), G.mx_decode(wc, ws), o)
+    ws[:, 1::2], xs[1::2] = 255, 255
+    y = ops.grouped_gemm(torch.from_numpy(xc).to(gpu), _stack(wc, ws, gpu), off, x_scales=torch.from_numpy(xs).to(gpu),
+                         out_dtype=torch.float32)
+    _equal(y[::2, ::2], ref[::2, ::2], "f32")
+    assert torch.isnan(y[1::2]).all() and torch.isnan(y[:, 1::2]).all()
+    x = _ints(rng, (P, K))
+    y = ops.grouped_gemm(_dev(x, "bf16", gpu), _stack(wc, ws, gpu), off, out_dtype=torch.float32)
+    ws[:, 1::2] = 127
+    _equal(y[:, ::2], G.forward(x, G.mx_decode(wc, ws), o)[:, ::2], "f32")
+    assert torch.isnan(y[:, 1::2]).all()
+
+
 @pytest.mark.parametrize("out,shift", [("bf16", 1), ("f16", 8), ("f32", 1)])
 @pytest.mark.parametrize("M", [1032, 4104])
 def test_element_alignment(gpu, M, out, shift):
