@@ -5,17 +5,17 @@
 // on MFMA (16 x 16 x 32, 16-bit operands; forward with both operands in MXFP4: the scaled
 // 16 x 16 x 128, four times the columns in the same bytes).
 //
-// A CTA is 4 waves (2 x 2) on a tile of 256 x 256, a wave 128 x 128 in 256 accumulation registers: 128
-// columns more than a wave of 8 would have need a third less from LDS for a product, whose
-// bandwidth held those back (60% of the matrix rate, 66% here, and 75% with the loads spread out).  Where that
-// leaves CUs without a tile: 128 x 128, two CTAs a CU.  K goes in stages of 128 bytes a row (64
+// A CTA is 4 waves (2 x 2) on a tile of 256 x 256, a wave 128 x 128 in 256 accumulation registers.  A product
+// reads 1/8 of two fragments from LDS there; on the 128 x 64 of 8 waves a half more, and LDS, which takes the
+// loads too, held those back (60% of the matrix rate).  Where such tiles leave CUs without one: 128 x 128, two
+// CTAs a CU.  K goes in stages of 128 bytes a row (64
 // columns, MXFP4: 256; whole cache lines, half lines cost a quarter of the time), two substeps each, through
 // rings of stages filled by 16-byte LDS DMA: two of the r operand, three (MXFP4: two) of
 // the c operand, whose first touch of a matrix comes from HBM.  A substep's fragments are
-// read among the products of the one before, a read or a load behind every second product: one wave a SIMD, whatever
-// is issued in a row there is time the matrix unit stands still.  One barrier a stage: behind the first products of
-// its second substep, when its last fragments are in registers; it frees the stage's slots and
-// hands over the next stage.
+// read while the one before is multiplied, a read or a load behind every second product: a wave alone on its SIMD
+// loses whatever is issued in a row (loads in one half of a stage only: 66% of the matrix rate in a long
+// reduction, spread out 75%).  One barrier a stage: behind the first products of its second substep, when its last
+// fragments are in registers; it frees the stage's slots and hands over the next stage.
 // Layouts of a stage (reads without bank conflicts):
 //   k-contiguous  128-byte rows, 16-byte chunk q of row r at q ^ (r / 2 % 8)
 //   transposed    rows of the tile's columns (chunk q of row r at q ^ (2 (r % 4) + 8 (r / 8 % 2))), read
